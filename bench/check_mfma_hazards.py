@@ -28,6 +28,8 @@ import tempfile
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "distributed_training_pytorch_amd", "csrc")
 HIPCC = "/opt/rocm/bin/hipcc"
+sys.path.insert(0, ROOT)
+from distributed_training_pytorch_amd._build import device_flags   # noqa: E402  (the flags the library is built with)
 
 REG = re.compile(r"\bv\[(\d+):(\d+)\]|\bv(\d+)\b")
 LABEL = re.compile(r"^([.\w$]+):")
@@ -128,8 +130,8 @@ def main():
 
         def to_asm(f):
             out = os.path.join(td, os.path.basename(f) + ".s")
-            return out, subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=fast", *defs,
-                                        "-I", CSRC, "-S", "--cuda-device-only", "-o", out, f], capture_output=True, text=True)
+            return out, subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=fast",
+                                        *device_flags(f), *defs, "-I", CSRC, "-S", "--cuda-device-only", "-o", out, f], capture_output=True, text=True)
         # the compilations are independent: run them side by side (igemm.hip alone takes a minute)
         import concurrent.futures
         with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(files), os.cpu_count() or 1)) as ex:
