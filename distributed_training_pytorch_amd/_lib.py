@@ -66,12 +66,19 @@ _SIGS = {
                               c_int, c_int, c_int, c_int, c_float, c_float, c_void_p, c_int, c_void_p],
     "dtp_bn_bwd_pool": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float,
                         c_float, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
+    "dtp_gn_workspace": [c_int, c_int, c_int, c_int, c_int, c_int],
+    "dtp_gn_fwd": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_int, c_int, c_int, c_int, c_int,
+                   c_int, c_float, c_void_p],
+    "dtp_gn_bwd": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float, c_float,
+                   c_void_p, c_size_t, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
     "dtp_augment_u8": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
     "dtp_sgd_flat": [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_size_t, c_float, c_float, c_float,
                      c_float, c_float, c_int, c_int, c_void_p],
     "dtp_adamw_flat": [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_float, c_float,
                        c_float, c_float, c_float, c_float, c_int, c_void_p],
 }
+
+_RESTYPES = {"dtp_gn_workspace": c_size_t}      # everything else returns an int status
 
 
 def lib_path(name="libdtp_hip.so"):
@@ -94,7 +101,7 @@ def _load(name, sigs):
             continue
         f = getattr(lib, fn)
         f.argtypes = args
-        f.restype = c_int
+        f.restype = _RESTYPES.get(fn, c_int)
     return lib
 
 

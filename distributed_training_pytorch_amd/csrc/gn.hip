@@ -1,0 +1,466 @@
+// Group normalisation + activation over channels-last activations [N][HW][C] for gfx950: per image n and group
+// g of C/G neighbouring channels, over the m = HW * C/G values of the group,
+//
+//   forward    mean, rstd = 1 / sqrt(var + eps);  xhat = (x - mean) * rstd;  y = act(xhat * gamma + beta)
+//   backward   dz = dy * act'(z);  dbeta = sum_{n,hw} dz;  dgamma = sum_{n,hw} dz * xhat
+//              dx = rstd * (gamma*dz - m1 - xhat*m2),  m1 = mean_group(gamma*dz),  m2 = mean_group(gamma*dz*xhat)
+//
+// x, y, dy, dx: bf16, f16 or f32; gamma, beta, statistics and every sum: f32 (folds of partial sums in f64);
+// one rounding, of the result.  Statistics of an image never leave it, so nothing is shared between images but
+// the gamma / beta gradients, which a last kernel sums in a fixed order (no atomics: results repeat bit for bit).
+//
+// Variance: sums of (x - p) and (x - p)^2 with p = the group's first value, so that a mean far from zero does not
+// cancel (E[x^2] - mean^2 in f32 loses mean^2 / var * 6e-8).
+#include "dtp_common.h"
+
+namespace {
+
+constexpr int GN_MAXC = 4096;        // channels: a block's per-channel sums live in LDS (2 * C floats)
+
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2 };
+
+struct tag_bf16 { static constexpr int size = 2; };
+struct tag_f16 { static constexpr int size = 2; };
+struct tag_f32 { static constexpr int size = 4; };
+
+// VEC values of one row as a machine word (2, 4, 8 or 16 bytes): one load, unpacked where it is used
+template <int BYTES> struct Word;
+template <> struct Word<2> { typedef uint16_t t; };
+template <> struct Word<4> { typedef uint32_t t; };
+template <> struct Word<8> { typedef u32x2_t t; };
+template <> struct Word<16> { typedef u32x4_t t; };
+
+template <class T, int VEC> struct Pack {
+  typedef typename Word<T::size * VEC>::t word;
+  DTP_DEVINL static uint32_t half_at(const word& w, int e) {
+    if constexpr (VEC == 1) return w;
+    else if constexpr (VEC == 2) return (w >> (16 * (e & 1))) & 0xFFFFu;
+    else return (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+  }
+  DTP_DEVINL static void unpack(const word& w, float* f) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      if constexpr (T::size == 4) {
+        if constexpr (VEC == 1) f[e] = __uint_as_float(w);
+        else f[e] = __uint_as_float(w[e]);
+      } else if constexpr (__is_same(T, tag_bf16)) {
+        f[e] = __uint_as_float(half_at(w, e) << 16);
+      } else {
+        f[e] = (float)__builtin_bit_cast(_Float16, (uint16_t)half_at(w, e));
+      }
+    }
+  }
+  DTP_DEVINL static uint32_t bits16(float f) {
+    if constexpr (__is_same(T, tag_bf16)) return f32_to_bf16(f);
+    else return __builtin_bit_cast(uint16_t, (_Float16)f);
+  }
+  DTP_DEVINL static word pack(const float* f) {
+    word w;
+    if constexpr (T::size == 4) {
+      if constexpr (VEC == 1) w = __float_as_uint(f[0]);
+      else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[e] = __float_as_uint(f[e]);
+      }
+    } else if constexpr (VEC == 1) {
+      w = (uint16_t)bits16(f[0]);
+    } else if constexpr (VEC == 2) {
+      w = bits16(f[0]) | (bits16(f[1]) << 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC / 2; ++e) {
+        if constexpr (__is_same(T, tag_bf16)) w[e] = pack_bf16x2(f[2 * e], f[2 * e + 1]);
+        else w[e] = bits16(f[2 * e]) | (bits16(f[2 * e + 1]) << 16);
+      }
+    }
+    return w;
+  }
+};
+
+// 1 / (1 + exp(-z)).  f32 results: the library's exp and an IEEE division.  16-bit results: the hardware's exp2 and
+// reciprocal (together < 4 units of f32's last place, 2^-13 of a bf16 step).
+template <class T> DTP_DEVINL float sigmoid(float z) {
+  if constexpr (T::size == 4) return 1.f / (1.f + expf(-z));
+  else return __builtin_amdgcn_rcpf(1.f + __expf(-z));
+}
+template <class T> DTP_DEVINL float act_fwd(float z, int act) {
+  if (act == ACT_RELU) return z <= 0.f ? 0.f : z;            // NaN stays NaN
+  if (act == ACT_SILU) return z * sigmoid<T>(z);
+  return z;
+}
+template <class T> DTP_DEVINL float act_bwd(float z, float dy, int act) {
+  if (act == ACT_RELU) return z > 0.f ? dy : 0.f;
+  if (act == ACT_SILU) {
+    const float s = sigmoid<T>(z);
+    return dy * s * (1.f + z * (1.f - s));
+  }
+  return dy;
+}
+
+DTP_DEVINL double wave_reduce_sum_f64(double v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+struct GnShape {
+  int N, HW, C, G, cpg;      // cpg = C / G
+  int CV;                    // C / VEC
+  int chunks, rows;          // an image's rows in `chunks` pieces of `rows`
+};
+
+// The value around which a group's sums are taken: its first one in the image.
+template <class T, int VEC>
+DTP_DEVINL float pivot_of(const typename Pack<T, VEC>::word* xn, int group, int cpg) {
+  float f;
+  Pack<T, 1>::unpack(((const typename Pack<T, 1>::word*)xn)[(size_t)group * cpg], &f);
+  return f;
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// Any size: partial sums over pieces of an image, a fold, and a second pass over the data.
+// A block's threads stand in rows of min(C / VEC, 256) columns; a thread keeps its column, so its channels'
+// parameters stay in registers.
+constexpr int GN_T = 256;
+
+// BWD 0: per group (sum (x-p), sum (x-p)^2) -> partial [N][chunks][G][2]
+// BWD 1: per channel (sum dz, sum dz*xhat)  -> partial [N][chunks][2][C]
+template <class T, int VEC, int BWD>
+__global__ __launch_bounds__(GN_T) void gn_partial_kernel(const void* __restrict__ x_, const void* __restrict__ dy_,
+                                                          const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                          const float* __restrict__ stats, float* __restrict__ partial,
+                                                          const GnShape s, const int act) {
+  typedef typename Pack<T, VEC>::word word;
+  extern __shared__ float sm[];                     // [2][C] channel sums, then [2][GN_T * VEC] thread sums
+  float* chs = sm;
+  float* thr = sm + 2 * s.C;
+  const int n = blockIdx.x / s.chunks, chunk = blockIdx.x - n * s.chunks;
+  const int r0 = chunk * s.rows, r1 = min(s.HW, r0 + s.rows);
+  const word* xn = (const word*)x_ + (size_t)n * s.HW * s.CV;
+  const word* dn = BWD ? (const word*)dy_ + (size_t)n * s.HW * s.CV : nullptr;
+  const int TX = min(s.CV, GN_T), R = GN_T / TX;
+  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+  for (int cb = 0; cb < s.CV; cb += TX) {
+    const int cv = cb + tx;
+    const bool on = ty < R && cv < s.CV;
+    float a0[VEC], a1[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) a0[e] = a1[e] = 0.f;
+    if (on) {
+      float p[VEC], rs[VEC], ga[VEC], be[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int c = cv * VEC + e, g = c / s.cpg;
+        if (BWD) {
+          p[e] = stats[((size_t)n * s.G + g) * 2];
+          rs[e] = stats[((size_t)n * s.G + g) * 2 + 1];
+          ga[e] = gamma[c];
+          be[e] = beta[c];
+        } else {
+          p[e] = pivot_of<T, VEC>(xn, g, s.cpg);
+        }
+      }
+#pragma unroll 4
+      for (int r = r0 + ty; r < r1; r += R) {
+        float f[VEC];
+        Pack<T, VEC>::unpack(xn[(size_t)r * s.CV + cv], f);
+        if (BWD) {
+          float d[VEC];
+          Pack<T, VEC>::unpack(dn[(size_t)r * s.CV + cv], d);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const float xh = (f[e] - p[e]) * rs[e];
+            const float dz = act_bwd<T>(fmaf(xh, ga[e], be[e]), d[e], act);
+            a0[e] += dz;
+            a1[e] = fmaf(dz, xh, a1[e]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const float d = f[e] - p[e];
+            a0[e] += d;
+            a1[e] = fmaf(d, d, a1[e]);
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        thr[(ty * TX + tx) * VEC + e] = a0[e];
+        thr[GN_T * VEC + (ty * TX + tx) * VEC + e] = a1[e];
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * TX * VEC; i += GN_T) {
+      const int which = i / (TX * VEC), j = i - which * TX * VEC, c = cb * VEC + j;
+      if (c < s.C) {
+        float t = 0.f;
+        for (int k = 0; k < R; ++k) t += thr[which * GN_T * VEC + k * TX * VEC + j];
+        if (BWD) partial[(((size_t)n * s.chunks + chunk) * 2 + which) * s.C + c] = t;
+        else chs[which * s.C + c] = t;
+      }
+    }
+    __syncthreads();
+  }
+  if (!BWD) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int g = wave; g < s.G; g += GN_T / 64) {
+      float u = 0.f, v = 0.f;
+      for (int c = lane; c < s.cpg; c += 64) {
+        u += chs[g * s.cpg + c];
+        v += chs[s.C + g * s.cpg + c];
+      }
+      u = wave_reduce_sum(u);
+      v = wave_reduce_sum(v);
+      if (lane == 0) {
+        float* o = partial + (((size_t)n * s.chunks + chunk) * s.G + g) * 2;
+        o[0] = u;
+        o[1] = v;
+      }
+    }
+  }
+}
+
+// mean and rstd of (image, group) from its pieces' sums: one wave each
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void gn_stats_kernel(const void* __restrict__ x_, const float* __restrict__ partial,
+                                                       float* __restrict__ stats, const GnShape s, const float eps) {
+  const long idx = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (idx >= (long)s.N * s.G) return;
+  const int n = (int)(idx / s.G), g = (int)(idx - (long)n * s.G);
+  double u = 0.0, v = 0.0;
+  for (int k = lane; k < s.chunks; k += 64) {
+    const float* o = partial + (((size_t)n * s.chunks + k) * s.G + g) * 2;
+    u += (double)o[0];
+    v += (double)o[1];
+  }
+  u = wave_reduce_sum_f64(u);
+  v = wave_reduce_sum_f64(v);
+  if (lane == 0) {
+    typedef typename Pack<T, VEC>::word word;
+    const double p = (double)pivot_of<T, VEC>((const word*)x_ + (size_t)n * s.HW * s.CV, g, s.cpg);
+    const double m = (double)s.HW * s.cpg, d = u / m;
+    double var = v / m - d * d;
+    if (var < 0.0) var = 0.0;
+    stats[idx * 2] = (float)(p + d);
+    stats[idx * 2 + 1] = (float)(1.0 / sqrt(var + (double)eps));
+  }
+}
+
+// Backward: per image, fold the pieces to per-channel sums [N][2][C] and per-group (m1, m2) [N][G][2]
+__global__ __launch_bounds__(256) void gn_bwd_fold_kernel(const float* __restrict__ partial,
+                                                          const float* __restrict__ gamma, float* __restrict__ sums,
+                                                          float* __restrict__ coef, const GnShape s) {
+  extern __shared__ float sm[];                     // [2][C]
+  const int n = blockIdx.x;
+  for (int i = threadIdx.x; i < 2 * s.C; i += 256) {
+    double t = 0.0;
+    for (int k = 0; k < s.chunks; ++k) t += (double)partial[((size_t)n * s.chunks + k) * 2 * s.C + i];
+    sums[(size_t)n * 2 * s.C + i] = (float)t;
+    sm[i] = (float)t * gamma[i >= s.C ? i - s.C : i];
+  }
+  __syncthreads();
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const float inv = 1.f / ((float)s.HW * (float)s.cpg);
+  for (int g = wave; g < s.G; g += 4) {
+    float u = 0.f, v = 0.f;
+    for (int c = lane; c < s.cpg; c += 64) {
+      u += sm[g * s.cpg + c];
+      v += sm[s.C + g * s.cpg + c];
+    }
+    u = wave_reduce_sum(u);
+    v = wave_reduce_sum(v);
+    if (lane == 0) {
+      coef[((size_t)n * s.G + g) * 2] = u * inv;
+      coef[((size_t)n * s.G + g) * 2 + 1] = v * inv;
+    }
+  }
+}
+
+// dgamma / dbeta: the images' channel sums [N][2][C], 16 channels a block, 16 strands of images a channel,
+// summed in f64 in a fixed order; written, or added to what is there (beta_* = 1)
+__global__ __launch_bounds__(256) void gn_dparam_kernel(const float* __restrict__ sums, int N, int C,
+                                                        void* __restrict__ dgamma, void* __restrict__ dbeta, int out_fp32,
+                                                        float beta_g, float beta_b) {
+  __shared__ double red[2][16][16];
+  const int ci = threadIdx.x & 15, part = threadIdx.x >> 4, c = blockIdx.x * 16 + ci;
+  double a = 0.0, b = 0.0;
+  if (c < C) {
+    for (int n = part; n < N; n += 16) {
+      a += (double)sums[((size_t)n * 2) * C + c];
+      b += (double)sums[((size_t)n * 2 + 1) * C + c];
+    }
+  }
+  red[0][part][ci] = a;
+  red[1][part][ci] = b;
+  __syncthreads();
+  if (part != 0 || c >= C) return;
+  a = b = 0.0;
+  for (int k = 0; k < 16; ++k) { a += red[0][k][ci]; b += red[1][k][ci]; }
+  if (out_fp32) {
+    float* dg = (float*)dgamma; float* db = (float*)dbeta;
+    dg[c] = (beta_g != 0.f ? beta_g * dg[c] : 0.f) + (float)b;
+    db[c] = (beta_b != 0.f ? beta_b * db[c] : 0.f) + (float)a;
+  } else {
+    bf16_t* dg = (bf16_t*)dgamma; bf16_t* db = (bf16_t*)dbeta;
+    dg[c] = f32_to_bf16((beta_g != 0.f ? beta_g * bf16_to_f32(dg[c]) : 0.f) + (float)b);
+    db[c] = f32_to_bf16((beta_b != 0.f ? beta_b * bf16_to_f32(db[c]) : 0.f) + (float)a);
+  }
+}
+
+template <class T, int VEC, int BWD>
+__global__ __launch_bounds__(GN_T) void gn_apply_kernel(const void* __restrict__ x_, const void* __restrict__ dy_,
+                                                        const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                        const float* __restrict__ stats, const float* __restrict__ coef,
+                                                        void* __restrict__ out_, const GnShape s, const int act) {
+  typedef typename Pack<T, VEC>::word word;
+  const int n = blockIdx.x / s.chunks, chunk = blockIdx.x - n * s.chunks;
+  const int r0 = chunk * s.rows, r1 = min(s.HW, r0 + s.rows);
+  const size_t base = (size_t)n * s.HW * s.CV;
+  const word* xn = (const word*)x_ + base;
+  const word* dn = BWD ? (const word*)dy_ + base : nullptr;
+  word* on = (word*)out_ + base;
+  const int TX = min(s.CV, GN_T), R = GN_T / TX;
+  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+  if (ty >= R) return;
+  for (int cv = tx; cv < s.CV; cv += TX) {
+    float mu[VEC], rs[VEC], ga[VEC], be[VEC], m1[VEC], m2[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int c = cv * VEC + e;
+      const size_t gi = ((size_t)n * s.G + c / s.cpg) * 2;
+      mu[e] = stats[gi];
+      rs[e] = stats[gi + 1];
+      ga[e] = gamma[c];
+      be[e] = beta[c];
+      if (BWD) { m1[e] = coef[gi]; m2[e] = coef[gi + 1]; }
+    }
+#pragma unroll 4
+    for (int r = r0 + ty; r < r1; r += R) {
+      float f[VEC], o[VEC];
+      Pack<T, VEC>::unpack(xn[(size_t)r * s.CV + cv], f);
+      if (BWD) {
+        float d[VEC];
+        Pack<T, VEC>::unpack(dn[(size_t)r * s.CV + cv], d);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float xh = (f[e] - mu[e]) * rs[e];
+          const float dz = act_bwd<T>(fmaf(xh, ga[e], be[e]), d[e], act);
+          o[e] = rs[e] * (fmaf(ga[e], dz, -m1[e]) - xh * m2[e]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o[e] = act_fwd<T>(fmaf((f[e] - mu[e]) * rs[e], ga[e], be[e]), act);
+      }
+      on[(size_t)r * s.CV + cv] = Pack<T, VEC>::pack(o);
+    }
+  }
+}
+
+// Pieces of an image: about 2,048 blocks in all (8 a CU), but no piece under 32 KB, where a block's fixed part
+// (parameters, LDS fold) would outweigh its rows.
+GnShape shape_of(int N, int HW, int C, int G, int vec, int elem) {
+  GnShape s;
+  s.N = N; s.HW = HW; s.C = C; s.G = G; s.cpg = C / G; s.CV = C / vec;
+  long want = (2048 + N - 1) / N;
+  const long most = ((long)HW * C * elem + 32767) / 32768;
+  if (want > most) want = most;
+  if (want > HW) want = HW;
+  if (want < 1) want = 1;
+  s.rows = (int)((HW + want - 1) / want);
+  s.chunks = (HW + s.rows - 1) / s.rows;
+  return s;
+}
+
+bool gn_ok(int N, int HW, int C, int G, int dtype, int act) {
+  return N > 0 && HW > 0 && C > 0 && C <= GN_MAXC && G > 0 && C % G == 0 && dtype >= 0 && dtype <= 2 && act >= 0 &&
+         act <= 2 && (long)HW * C < 0x7fffffffL && (long)N * HW < 0x7fffffffL;
+}
+
+// widest vector of at most 16 bytes that divides a row
+int gn_vec(int C, int elem) {
+  int v = 16 / elem;
+  while (C % v) v >>= 1;
+  return v;
+}
+
+size_t partial_floats(const GnShape& s, int bwd) {
+  return bwd ? (size_t)s.N * s.chunks * 2 * s.C : (size_t)s.N * s.chunks * s.G * 2;
+}
+
+template <class T, int VEC>
+int gn_run_fwd(const void* x, const float* gamma, const float* beta, void* y, float* stats, float* ws, size_t ws_floats,
+               const GnShape& s, float eps, int act, hipStream_t st) {
+  if (ws_floats < partial_floats(s, 0)) return -12;
+  const size_t lds = (size_t)(2 * s.C + 2 * GN_T * VEC) * sizeof(float);
+  const dim3 grid(s.N * s.chunks);
+  hipLaunchKernelGGL((gn_partial_kernel<T, VEC, 0>), grid, dim3(GN_T), lds, st, x, nullptr, gamma, beta, nullptr, ws, s, act);
+  hipLaunchKernelGGL((gn_stats_kernel<T, VEC>), dim3((unsigned)(((long)s.N * s.G + 3) / 4)), dim3(256), 0, st, x, ws, stats, s, eps);
+  hipLaunchKernelGGL((gn_apply_kernel<T, VEC, 0>), grid, dim3(GN_T), 0, st, x, nullptr, gamma, beta, stats, nullptr, y, s, act);
+  return DTP_CHECK_LAUNCH();
+}
+
+template <class T, int VEC>
+int gn_run_bwd(const void* x, const void* dy, const float* gamma, const float* beta, const float* stats, void* dx,
+               void* dgamma, void* dbeta, int out_fp32, float beta_g, float beta_b, float* ws, size_t ws_floats,
+               const GnShape& s, int act, hipStream_t st) {
+  const size_t np = partial_floats(s, 1), ns = (size_t)s.N * 2 * s.C, nc = (size_t)s.N * s.G * 2;
+  if (ws_floats < np + ns + nc) return -12;
+  float *sums = ws + np, *coef = sums + ns;
+  const size_t lds = (size_t)(2 * s.C + 2 * GN_T * VEC) * sizeof(float);
+  const dim3 grid(s.N * s.chunks);
+  hipLaunchKernelGGL((gn_partial_kernel<T, VEC, 1>), grid, dim3(GN_T), lds, st, x, dy, gamma, beta, stats, ws, s, act);
+  hipLaunchKernelGGL(gn_bwd_fold_kernel, dim3(s.N), dim3(256), (size_t)2 * s.C * sizeof(float), st, ws, gamma, sums, coef, s);
+  hipLaunchKernelGGL((gn_apply_kernel<T, VEC, 1>), grid, dim3(GN_T), 0, st, x, dy, gamma, beta, stats, coef, dx, s, act);
+  hipLaunchKernelGGL(gn_dparam_kernel, dim3((s.C + 15) / 16), dim3(256), 0, st, sums, s.N, s.C, dgamma, dbeta, out_fp32,
+                     beta_g, beta_b);
+  return DTP_CHECK_LAUNCH();
+}
+
+}  // namespace
+
+#define GN_DISPATCH(FN, ...)                                      \
+  do {                                                            \
+    if (dtype == 2) {                                             \
+      if (vec == 4) return FN<tag_f32, 4>(__VA_ARGS__);           \
+      if (vec == 2) return FN<tag_f32, 2>(__VA_ARGS__);           \
+      return FN<tag_f32, 1>(__VA_ARGS__);                         \
+    }                                                             \
+    if (dtype == 1) {                                             \
+      if (vec == 8) return FN<tag_f16, 8>(__VA_ARGS__);           \
+      if (vec == 4) return FN<tag_f16, 4>(__VA_ARGS__);           \
+      if (vec == 2) return FN<tag_f16, 2>(__VA_ARGS__);           \
+      return FN<tag_f16, 1>(__VA_ARGS__);                         \
+    }                                                             \
+    if (vec == 8) return FN<tag_bf16, 8>(__VA_ARGS__);            \
+    if (vec == 4) return FN<tag_bf16, 4>(__VA_ARGS__);            \
+    if (vec == 2) return FN<tag_bf16, 2>(__VA_ARGS__);            \
+    return FN<tag_bf16, 1>(__VA_ARGS__);                          \
+  } while (0)
+
+// Floats of scratch that dtp_gn_fwd (bwd = 0) / dtp_gn_bwd (bwd = 1) need; 0: shape refused.
+extern "C" size_t dtp_gn_workspace(int N, int HW, int C, int G, int dtype, int bwd) {
+  if (!gn_ok(N, HW, C, G, dtype, 0)) return 0;
+  const int elem = dtype == 2 ? 4 : 2;
+  const GnShape s = shape_of(N, HW, C, G, gn_vec(C, elem), elem);
+  return partial_floats(s, bwd) + (bwd ? (size_t)N * 2 * C + (size_t)N * G * 2 : 0);
+}
+
+// x, y: [N][HW][C] (dtype 0 bf16, 1 f16, 2 f32), 16-byte aligned; gamma, beta: f32 [C]; stats: f32 [N][G][2] (mean, rstd)
+extern "C" int dtp_gn_fwd(const void* x, const float* gamma, const float* beta, void* y, float* stats, float* ws,
+                          size_t ws_floats, int N, int HW, int C, int G, int dtype, int act, float eps, hipStream_t st) {
+  if (!gn_ok(N, HW, C, G, dtype, act)) return -10;
+  const int elem = dtype == 2 ? 4 : 2, vec = gn_vec(C, elem);
+  const GnShape s = shape_of(N, HW, C, G, vec, elem);
+  GN_DISPATCH(gn_run_fwd, x, gamma, beta, y, stats, ws, ws_floats, s, eps, act, st);
+}
+
+// stats as dtp_gn_fwd left them; dgamma / dbeta: [C], f32 or bf16, written (beta_* = 0) or added to (beta_* = 1)
+extern "C" int dtp_gn_bwd(const void* x, const void* dy, const float* gamma, const float* beta, const float* stats,
+                          void* dx, void* dgamma, void* dbeta, int out_fp32, float beta_g, float beta_b, float* ws,
+                          size_t ws_floats, int N, int HW, int C, int G, int dtype, int act, hipStream_t st) {
+  if (!gn_ok(N, HW, C, G, dtype, act)) return -10;
+  const int elem = dtype == 2 ? 4 : 2, vec = gn_vec(C, elem);
+  const GnShape s = shape_of(N, HW, C, G, vec, elem);
+  GN_DISPATCH(gn_run_bwd, x, dy, gamma, beta, stats, dx, dgamma, dbeta, out_fp32, beta_g, beta_b, ws, ws_floats, s, act, st);
+}

@@ -6,6 +6,7 @@ launches on the caller's current HIP stream.  Tensors are internal-layout: activ
 ``[N, H, W, C]``, conv weights ``[Cout, 9*Cin]`` (tap-major, channel-minor), linear weights
 ``[out, in]``.
 """
+import contextlib as _contextlib
 import ctypes as _ctypes
 import os as _os
 
@@ -955,6 +956,90 @@ def bn_bwd_pool(y, dzp, codes, gamma, stats, dgamma, dbeta, beta_g=0.0, beta_b=0
                                      ptr(dbeta), int(dgamma.dtype == torch.float32), float(beta_g), float(beta_b),
                                      ptr(part), ptr(work), N, H, W, C, stream()), "bn_bwd_pool")
     return dy
+
+
+GN_DTYPES = {BF16: 0, torch.float16: 1, torch.float32: 2}
+GN_ACTS = {"none": 0, "relu": 1, "silu": 2}
+
+
+def _on_device_of(t):
+    """The launch goes to the current stream of the tensors' own device, whatever device is current."""
+    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else _contextlib.nullcontext()
+
+
+def _gn_check(x, groups, act, *vecs):
+    if not torch.is_tensor(x) or x.dtype not in GN_DTYPES:
+        raise ValueError("group norm: x must be a bf16, f16 or f32 tensor")
+    if x.dim() < 2:
+        raise ValueError("group norm: x must be [N, ..., C], got %s" % (tuple(x.shape),))
+    if act not in GN_ACTS:
+        raise ValueError("group norm: act must be one of %s, got %r" % (sorted(GN_ACTS), act))
+    N, C, G = x.shape[0], x.shape[-1], int(groups)
+    if G < 1 or C < 1 or C % G or C > 4096:
+        raise ValueError("group norm: %d channels in %d groups (channels must be a multiple of groups, at most 4096)" % (C, G))
+    HW = 1
+    for d in x.shape[1:-1]:
+        HW *= d
+    if HW == 0 and N > 0:
+        raise ValueError("group norm: no values to normalise in %s" % (tuple(x.shape),))
+    if HW * C >= 2 ** 31 - 1 or N * HW >= 2 ** 31 - 1:
+        raise ValueError("group norm: %s is too large (2^31 values an image, 2^31 pixels)" % (tuple(x.shape),))
+    for v in vecs:
+        if v.dtype != torch.float32 or not v.is_contiguous() or v.numel() != C or v.device != x.device:
+            raise ValueError("group norm: gamma / beta must be contiguous f32 [C] on x's device")
+    _need(x, x.dtype, "x")
+    return N, HW, C, G
+
+
+def gn_fwd(x, gamma, beta, groups, eps=1e-5, act="relu"):
+    """y = act(group_norm(x)) over channels-last x [N, ..., C] (bf16, f16 or f32, contiguous): per image and
+    group of C / groups neighbouring channels, mean and variance over all positions; gamma / beta f32 [C];
+    act "none", "relu" or "silu".  Returns (y, stats), stats f32 [N, groups, 2] = (mean, 1 / sqrt(var + eps))
+    for :func:`gn_bwd`."""
+    N, HW, C, G = _gn_check(x, groups, act, gamma, beta)
+    y = torch.empty_like(x)
+    stats = torch.empty((N, G, 2), dtype=torch.float32, device=x.device)
+    if N == 0:
+        return y, stats
+    dt = GN_DTYPES[x.dtype]
+    lib = _lib.hip()
+    with _on_device_of(x):
+        # scratch of this call alone (the caching allocator's, so a captured graph keeps its own): calls on two
+        # streams, or two graphs, share nothing
+        ws = torch.empty(lib.dtp_gn_workspace(N, HW, C, G, dt, 0), dtype=torch.float32, device=x.device)
+        check(lib.dtp_gn_fwd(ptr(x), ptr(gamma), ptr(beta), ptr(y), ptr(stats), ptr(ws), ws.numel(), N, HW, C, G, dt,
+                             GN_ACTS[act], float(eps), stream()), "gn_fwd")
+    return y, stats
+
+
+def gn_bwd(x, dy, gamma, beta, stats, groups, dgamma, dbeta, act="relu", beta_g=0.0, beta_b=0.0):
+    """dx of :func:`gn_fwd` given its input, its ``stats`` and dy (x's shape and type); dgamma / dbeta ([C], f32
+    or bf16, same dtype) are written (beta_* = 0) or accumulated into (beta_* = 1)."""
+    if dy.shape != x.shape or dy.device != x.device or dy.dtype != x.dtype:
+        raise ValueError("gn_bwd: dy must have x's shape, type and device")
+    N, HW, C, G = _gn_check(x, groups, act, gamma, beta)
+    _need(dy, x.dtype, "dy")
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (N, G, 2) or not stats.is_contiguous() or stats.device != x.device:
+        raise ValueError("gn_bwd: stats must be gn_fwd's [N, groups, 2] f32")
+    if dgamma.dtype != dbeta.dtype or dgamma.dtype not in (torch.float32, BF16) or dgamma.numel() != C \
+            or dbeta.numel() != C or not dgamma.is_contiguous() or not dbeta.is_contiguous() \
+            or dgamma.device != x.device or dbeta.device != x.device:
+        raise ValueError("gn_bwd: dgamma / dbeta must be contiguous [C] of one dtype (f32 / bf16) on x's device")
+    dx = torch.empty_like(x)
+    if N == 0:
+        if beta_g == 0.0:
+            dgamma.zero_()
+        if beta_b == 0.0:
+            dbeta.zero_()
+        return dx
+    dt = GN_DTYPES[x.dtype]
+    lib = _lib.hip()
+    with _on_device_of(x):
+        ws = torch.empty(lib.dtp_gn_workspace(N, HW, C, G, dt, 1), dtype=torch.float32, device=x.device)
+        check(lib.dtp_gn_bwd(ptr(x), ptr(dy), ptr(gamma), ptr(beta), ptr(stats), ptr(dx), ptr(dgamma), ptr(dbeta),
+                             int(dgamma.dtype == torch.float32), float(beta_g), float(beta_b), ptr(ws), ws.numel(), N, HW,
+                             C, G, dt, GN_ACTS[act], stream()), "gn_bwd")
+    return dx
 
 
 def cast_f32_bf16(src, dst):

@@ -1,0 +1,256 @@
+"""Group norm + activation (csrc/gn.hip) against the definition in 64 bits.
+
+Tolerances, per value: half a step of the output type (``eps / 2`` relative), and for the f32 arithmetic
+``L * 2^-24`` of the magnitudes that enter, with L = the longest chain of f32 additions a sum goes through (a thread
+adds at most 256 rows in these shapes, then 16 terms of a fold at most per level) plus 16 single operations.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+U = 2.0 ** -24
+
+
+def _k():
+    from distributed_training_pytorch_amd.ops import kernels
+    return kernels
+
+
+def _act(z, act):
+    if act == "relu":
+        return z.clamp_min(0)
+    return z * torch.sigmoid(z) if act == "silu" else z
+
+
+def _ref_stats(x, groups, eps):
+    n, c = x.shape[0], x.shape[-1]
+    v = x.double().reshape(n, -1, groups, c // groups)
+    mean = v.mean((1, 3))
+    var = v.var((1, 3), unbiased=False)
+    return mean, (var + eps).rsqrt(), v.abs().mean((1, 3)) + mean.abs()
+
+
+def _ref(x, gamma, beta, groups, eps, act):
+    n, c = x.shape[0], x.shape[-1]
+    v = x.double().reshape(n, -1, groups, c // groups)
+    mean, rstd, _ = _ref_stats(x, groups, eps)
+    xh = ((v - mean[:, None, :, None]) * rstd[:, None, :, None]).reshape(x.shape)
+    z = xh * gamma.double() + beta.double()
+    return _act(z, act), xh, z
+
+
+def _ref_bwd(x, dy, gamma, beta, groups, eps, act):
+    n, c = x.shape[0], x.shape[-1]
+    _, xh, z = _ref(x, gamma, beta, groups, eps, act)
+    _, rstd, _ = _ref_stats(x, groups, eps)
+    d = dy.double()
+    if act == "relu":
+        dz = d * (z > 0)
+    elif act == "silu":
+        s = torch.sigmoid(z)
+        dz = d * (s + z * s * (1 - s))
+    else:
+        dz = d
+    dims = tuple(range(x.dim() - 1))
+    dgamma, dbeta = (dz * xh).sum(dims), dz.sum(dims)
+    e, xg = (dz * gamma.double()).reshape(n, -1, groups, c // groups), xh.reshape(n, -1, groups, c // groups)
+    m1, m2 = e.mean((1, 3), keepdim=True), (e * xg).mean((1, 3), keepdim=True)
+    dx = ((e - m1 - xg * m2) * rstd[:, None, :, None]).reshape(x.shape)
+    mag = ((e.abs() + e.abs().mean((1, 3), keepdim=True) + xg.abs() * (e * xg).abs().mean((1, 3), keepdim=True))
+           * rstd[:, None, :, None]).reshape(x.shape)
+    return dx, dgamma, dbeta, mag, (dz * xh).abs().sum(dims), dz.abs().sum(dims)
+
+
+def _inputs(shape, dtype, seed=0, shift=0.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    c = shape[-1]
+    x = (torch.randn(shape, generator=g, device="cuda") * (0.5 + torch.rand(c, generator=g, device="cuda"))
+         + 0.5 * torch.randn(c, generator=g, device="cuda") + shift).to(dtype)
+    dy = torch.randn(shape, generator=g, device="cuda").to(dtype)
+    gamma = 1 + 0.3 * torch.randn(c, generator=g, device="cuda")
+    beta = 0.3 * torch.randn(c, generator=g, device="cuda")
+    return x, dy, gamma, beta
+
+
+def _check(got, ref, mag, name, chain=288):
+    tol = torch.finfo(got.dtype).eps / 2 * ref.abs() + chain * U * mag
+    if got.dtype == F16:
+        tol = tol + 2.0 ** -25          # half a step of its subnormals
+    err = (got.double() - ref).abs()
+    worst = (err / tol.clamp_min(1e-300)).max().item() if got.numel() else 0.0
+    assert worst <= 1.0, "%s: an element is %.2f times its tolerance off" % (name, worst)
+
+
+SHAPES = [  # shape, groups
+    ((1, 1, 1, 8), 8),              # one value a group: variance zero
+    ((2, 1, 1, 64), 4),             # one pixel
+    ((3, 64), 16),                  # no spatial axes
+    ((2, 3, 5, 7), 1),              # all channels one group, odd channels
+    ((4, 14, 14, 512), 32),
+    ((2, 28, 28, 512), 32),
+    ((2, 56, 56, 256), 32),
+    ((1, 112, 112, 128), 32),
+    ((2, 27, 19, 60), 12),
+    ((3, 9, 33, 36), 12),           # three channels a group
+    ((2, 17, 13, 96), 96),          # a group a channel
+    ((1, 7, 5, 2058), 3),           # wide rows
+    ((1, 2, 3, 4096), 2),
+    ((300, 2, 2, 16), 4),           # many small images
+    ((2, 1001, 24), 4),             # one long axis
+]
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "silu"])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("shape,groups", SHAPES)
+def test_gn_fwd(shape, groups, dtype, act):
+    k = _k()
+    x, _, gamma, beta = _inputs(shape, dtype)
+    y, stats = k.gn_fwd(x, gamma, beta, groups, eps=1e-5, act=act)
+    ref, xh, z = _ref(x, gamma, beta, groups, 1e-5, act)
+    mean, rstd, mag = _ref_stats(x, groups, 1e-5)
+    _check(stats[..., 0], mean, mag, "mean")
+    # var is off by chain * U of E[(x - p)^2] <= 2 (var + (mean - p)^2); here |mean - p| <= 6 std: rstd by half of that
+    _check(stats[..., 1], rstd, rstd * 40 * (1 + 0 * mag), "rstd")
+    # |dy/dz| <= 1.1; xhat is off by the statistics' errors and its own three operations
+    zmag = gamma.double().abs() * (xh.abs() * 40 + (mag * rstd).repeat_interleave(shape[-1] // groups, -1).view(
+        (shape[0],) + (1,) * (len(shape) - 2) + (shape[-1],))) + beta.double().abs()
+    _check(y, ref, 1.1 * zmag, "y")
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "silu"])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("shape,groups", SHAPES)
+def test_gn_bwd(shape, groups, dtype, act):
+    k = _k()
+    x, dy, gamma, beta = _inputs(shape, dtype, seed=1)
+    mean, rstd, _ = _ref_stats(x, groups, 1e-5)
+    stats = torch.stack((mean, rstd), -1).float()
+    if act == "relu":                        # keep gradients away from signs that f32 cannot decide
+        z = _ref(x, gamma, beta, groups, 1e-5, act)[2]
+        dy = torch.where(z.abs() > 1e-4, dy, torch.zeros_like(dy))
+    dg, db = torch.empty(shape[-1], device="cuda"), torch.empty(shape[-1], device="cuda")
+    dx = k.gn_bwd(x, dy, gamma, beta, stats, groups, dg, db, act=act)
+    rdx, rdg, rdb, mag, mg, mb = _ref_bwd(x, dy, gamma, beta, groups, 1e-5, act)
+    zmag = 1 + _ref(x, gamma, beta, groups, 1e-5, act)[2].abs().amax().item()      # d(act')/dz <= 1: its slope enters
+    extra = (x.double().abs().amax() + 1) * rstd.amax()                          # rounding of x - mean, per unit of xhat
+    _check(dx, rdx, mag * (zmag + extra), "dx")
+    _check(dg, rdg, mg * zmag + mb * extra, "dgamma")
+    _check(db, rdb, mb * (zmag + extra), "dbeta")
+
+
+def test_gn_mean_far_from_zero():
+    """mean / std = 1000 in f32: E[x^2] - mean^2 would lose 1e6 * 2^-24 = 6 % of the variance."""
+    k = _k()
+    x, _, gamma, beta = _inputs((2, 31, 17, 48), F32, shift=1000.0)
+    y, stats = k.gn_fwd(x, gamma, beta, 6, act="none")
+    ref, xh, _ = _ref(x, gamma, beta, 6, 1e-5, "none")
+    mean, rstd, _ = _ref_stats(x, 6, 1e-5)
+    # rstd: relative chain * U * E[(x-p)^2] / var <= 288 * U * 40; the mean: half a step of 1000
+    _check(stats[..., 1], rstd, rstd * 40, "rstd")
+    assert ((stats[..., 0].double() - mean).abs() <= 1000 * 2 * U + 288 * U * 3).all()
+    assert ((y.double() - ref).abs() <= 4 * 1000 * U * rstd.max() * gamma.abs().max() + 288 * U * 40 * (1 + ref.abs())).all()
+
+
+def test_gn_poison_stays_in_its_group():
+    k = _k()
+    x, dy, gamma, beta = _inputs((3, 8, 8, 32), F32)
+    clean, _ = k.gn_fwd(x, gamma, beta, 4, act="relu")
+    x2 = x.clone()
+    x2[1, 3, 2, 9] = float("nan")       # group 1 of image 1
+    x2[2, 0, 0, 31] = float("inf")      # group 3 of image 2
+    y, stats = k.gn_fwd(x2, gamma, beta, 4, act="relu")
+    bad = torch.zeros_like(x, dtype=torch.bool)
+    bad[1, :, :, 8:16] = True
+    bad[2, :, :, 24:] = True
+    assert torch.isnan(y[bad]).all() and torch.equal(y[~bad], clean[~bad])
+    dg, db = torch.empty(32, device="cuda"), torch.empty(32, device="cuda")
+    dx = k.gn_bwd(x2, dy, gamma, beta, stats, 4, dg, db, act="none")
+    assert torch.isfinite(dx[~bad]).all() and torch.isnan(dx[bad]).all()
+
+
+@pytest.mark.parametrize("gdtype", [F32, BF16])
+def test_gn_param_gradients_accumulate(gdtype):
+    k = _k()
+    x, dy, gamma, beta = _inputs((3, 11, 6, 40), BF16, seed=2)
+    y, stats = k.gn_fwd(x, gamma, beta, 5, act="silu")
+    dg0, db0 = torch.full((40,), 7.0, device="cuda", dtype=gdtype), torch.full((40,), -3.0, device="cuda", dtype=gdtype)
+    dg, db = torch.empty(40, device="cuda", dtype=gdtype), torch.empty(40, device="cuda", dtype=gdtype)
+    a = k.gn_bwd(x, dy, gamma, beta, stats, 5, dg, db, act="silu")
+    b = k.gn_bwd(x, dy, gamma, beta, stats, 5, dg0, db0, act="silu", beta_g=1.0, beta_b=1.0)
+    assert torch.equal(a, b)
+    e = torch.finfo(gdtype).eps
+    for once, more, was in ((dg, dg0, 7.0), (db, db0, -3.0)):
+        want = once.double() + was
+        assert ((more.double() - want).abs() <= e * (once.double().abs() + want.abs())).all()
+
+
+def test_gn_gradient_against_differences():
+    k = _k()
+    x, dy, gamma, beta = _inputs((2, 4, 5, 12), F32, seed=3)
+    _, stats = k.gn_fwd(x, gamma, beta, 3, act="silu")
+    dg, db = torch.empty(12, device="cuda"), torch.empty(12, device="cuda")
+    dx = k.gn_bwd(x, dy, gamma, beta, stats, 3, dg, db, act="silu")
+    g = torch.Generator(device="cuda").manual_seed(9)
+
+    def loss(x_, ga, be):
+        return (k.gn_fwd(x_, ga, be, 3, act="silu")[0].double() * dy.double()).sum().item()
+
+    h = 2.0 ** -6
+    for t, grad, put in ((x, dx, 0), (gamma, dg, 1), (beta, db, 2)):
+        v = torch.randn(t.shape, generator=g, device="cuda")
+        v = v / v.norm()
+        args = [x, gamma, beta]
+        up, down = list(args), list(args)
+        up[put], down[put] = t + h * v, t - h * v
+        fd = (loss(*up) - loss(*down)) / (2 * h)
+        want = (grad.double() * v.double()).sum().item()
+        # third-order term h^2/6 |f'''| with |f'''| <~ 10 |dy|_1-ish directions of unit length, and rounding 2^-20 / h
+        assert abs(fd - want) <= 10 * h * h + 480 * 2.0 ** -22 / h, (put, fd, want)
+
+
+def test_gn_repeats_bit_for_bit_on_streams_and_in_graphs():
+    k = _k()
+    x, dy, gamma, beta = _inputs((5, 27, 19, 64), BF16, seed=4)
+
+    def both(x_, dy_):
+        y, st = k.gn_fwd(x_, gamma, beta, 8, act="relu")
+        dg, db = torch.empty(64, device="cuda"), torch.empty(64, device="cuda")
+        return y, st, k.gn_bwd(x_, dy_, gamma, beta, st, 8, dg, db, act="relu"), dg, db
+
+    first = both(x, dy)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = both(x, dy)
+    again = both(x, dy)                         # on the default stream, next to the other one
+    torch.cuda.synchronize()
+    for a, b, c in zip(first, other, again):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    xs, graphs = [x.clone(), torch.flip(x, (0,)).contiguous()], []
+    for v in xs:                                # two graphs share no scratch
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            out = both(v, dy)
+        graphs.append((g, out))
+    for rep in range(3):
+        for v, (g, out) in zip(xs, graphs):
+            v.mul_(0.5 if rep == 1 else 1.0)
+            g.replay()
+        for v, (g, out) in zip(xs, graphs):
+            for a, b in zip(out, both(v, dy)):
+                assert torch.equal(a, b)
+
+
+def test_gn_empty_batch():
+    k = _k()
+    ga = torch.ones(16, device="cuda")
+    x = torch.empty((0, 4, 4, 16), device="cuda")
+    y, st = k.gn_fwd(x, ga, ga, 4)
+    dg, db = torch.full((16,), 5.0, device="cuda"), torch.full((16,), 5.0, device="cuda")
+    dx = k.gn_bwd(x, x, ga, ga, st, 4, dg, db, beta_b=1.0)
+    assert y.shape == x.shape == dx.shape and st.shape == (0, 4, 2)
+    assert (dg == 0).all() and (db == 5).all()
