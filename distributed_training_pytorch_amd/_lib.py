@@ -71,6 +71,11 @@ _SIGS = {
                    c_int, c_float, c_void_p],
     "dtp_gn_bwd": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float, c_float,
                    c_void_p, c_size_t, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
+    "dtp_ns_workspace": [c_int, c_void_p, c_void_p],
+    "dtp_newton_schulz": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_float,
+                          c_void_p, c_size_t, c_void_p],
+    "dtp_muon_step": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float, c_int, c_float,
+                      c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float, c_void_p, c_size_t, c_void_p],
     "dtp_augment_u8": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
     "dtp_sgd_flat": [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_size_t, c_float, c_float, c_float,
                      c_float, c_float, c_int, c_int, c_void_p],
@@ -78,7 +83,7 @@ _SIGS = {
                        c_float, c_float, c_float, c_float, c_int, c_void_p],
 }
 
-_RESTYPES = {"dtp_gn_workspace": c_size_t}      # everything else returns an int status
+_RESTYPES = {"dtp_gn_workspace": c_size_t, "dtp_ns_workspace": c_size_t}      # everything else returns an int status
 
 
 def lib_path(name="libdtp_hip.so"):

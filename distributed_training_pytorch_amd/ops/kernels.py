@@ -8,6 +8,8 @@ launches on the caller's current HIP stream.  Tensors are internal-layout: activ
 """
 import contextlib as _contextlib
 import ctypes as _ctypes
+import functools as _functools
+import math as _math
 import os as _os
 
 import torch
@@ -1116,3 +1118,180 @@ def adamw_flat(p, g, m, v, lp, lr, beta1, beta2, eps, wd, grad_scale, step):
                                    float(beta1), float(beta2), float(eps), float(wd), float(grad_scale), int(step),
                                    stream())
     check(rc, "adamw_flat")
+
+
+# ------------------------------------------------------------------------------------- Muon
+NS_COEFFS = (3.4445, -4.7750, 2.0315)
+NS_DTYPES = {torch.float32: 0, BF16: 1, torch.float16: 2}
+NS_MAX_STEPS = 12
+_NS_MAXMAT = 24                 # matrices per native call (csrc/muon.hip)
+
+
+@_functools.lru_cache(maxsize=64)
+def _ns_plan(steps, coeffs):
+    """(ctypes coefficients, ctypes scales) of the polynomial chain in csrc/muon.hip: for every segment's X and its
+    steps' A, P, Q the power of two that puts the matrix's largest possible entry (its spectral norm, over all
+    singular values in [0, 1] that X_0 can have) at 4096..8192 of f16's 65504."""
+    a, b, c = coeffs
+    n = 1 << 14
+    x = [i / n for i in range(n + 1)]
+
+    def pow2(bound):
+        return 2.0 ** _math.floor(_math.log2(8192.0 / max(bound, 2.0 ** -10)))
+
+    scales = []
+    for length in ns_segments(steps):
+        scales.append(pow2(max(abs(v) for v in x)))
+        q = [1.0] * (n + 1)
+        for _ in range(length):
+            lam = [v * v for v in x]
+            p = [a + b * v + c * v * v for v in lam]
+            nx = [v * w for v, w in zip(x, p)]
+            q = [v * w for v, w in zip(q, p)]
+            if not all(abs(v) <= 4.0 for v in nx):
+                raise ValueError("newton_schulz: coefficients %s drive singular values in [0, 1] past 4: the iteration "
+                                 "does not stay bounded" % (coeffs,))
+            scales += [pow2(max(max(lam), max(abs(v * w) for v, w in zip(x, nx)))), pow2(max(abs(v) for v in p)),
+                       pow2(max(abs(v) for v in q))]
+            x = nx
+    return (_ctypes.c_float * 3)(*coeffs), (_ctypes.c_float * len(scales))(*scales)
+
+
+def ns_segments(steps):
+    """Steps of each segment of the chain: at most three, as even as they go, longer ones first (csrc/muon.hip)."""
+    n = (steps + 2) // 3
+    return [steps // n + (1 if i < steps % n else 0) for i in range(n)]
+
+
+def _ns_check_schedule(steps, coeffs, eps):
+    if int(steps) != steps or not 1 <= steps <= NS_MAX_STEPS:
+        raise ValueError("newton_schulz: steps must be 1..%d, got %r" % (NS_MAX_STEPS, steps))
+    if len(coeffs) != 3 or not all(_math.isfinite(v) for v in coeffs):
+        raise ValueError("newton_schulz: coeffs must be three finite numbers, got %r" % (coeffs,))
+    if not (_math.isfinite(eps) and eps > 0):
+        raise ValueError("newton_schulz: eps must be positive, got %r" % (eps,))
+    return _ns_plan(int(steps), tuple(float(v) for v in coeffs))
+
+
+def _ns_check_sides(rows, cols):
+    if rows > 1 << 20 or cols > 1 << 20:
+        raise ValueError("newton_schulz: sides up to 2^20, got %d x %d" % (rows, cols))
+
+
+def _ints(v):
+    return (_ctypes.c_int * len(v))(*v)
+
+
+def _floats(v):
+    return (_ctypes.c_float * len(v))(*v)
+
+
+def _ptrs(v):
+    return (_ctypes.c_void_p * len(v))(*v)
+
+
+def newton_schulz(x, steps=5, coeffs=NS_COEFFS, eps=1e-7, out_dtype=None):
+    """Orthogonalise matrices by ``steps`` Newton-Schulz iterations: X = x / (|x|_F + eps), then
+    X = a X + (b S + c S^2) X with S = X X^T (``coeffs`` = a, b, c).  ``x``: [rows, cols], a stack
+    [batch, rows, cols], or a list of 2-D tensors of any shapes (one type: f32, bf16 or f16; contiguous);
+    returns the same structure in ``out_dtype`` (default: x's).  The products run on pairs of f16 values (22
+    bits), whatever the types: before its rounding the result is as near the exact one as a loop of f32 products'."""
+    many = isinstance(x, (list, tuple))
+    mats = list(x) if many else [x]
+    cf, sc = _ns_check_schedule(steps, coeffs, eps)
+    if not mats:
+        return []
+    first = mats[0]
+    if not torch.is_tensor(first) or first.dtype not in NS_DTYPES:
+        raise ValueError("newton_schulz: f32, bf16 or f16 tensors")
+    out_dtype = first.dtype if out_dtype is None else out_dtype
+    if out_dtype not in NS_DTYPES:
+        raise ValueError("newton_schulz: out_dtype must be f32, bf16 or f16, got %s" % (out_dtype,))
+    for t in mats:
+        if not torch.is_tensor(t) or t.dtype != first.dtype or t.device != first.device:
+            raise ValueError("newton_schulz: matrices of one type on one device")
+        if t.dim() != 2 and (many or t.dim() != 3):
+            raise ValueError("newton_schulz: [rows, cols], [batch, rows, cols] or a list of matrices, got %s" % (tuple(t.shape),))
+        if not t.is_contiguous():
+            raise ValueError("newton_schulz: matrices must be contiguous")
+        _ns_check_sides(t.shape[-2], t.shape[-1])
+    if not first.is_cuda:
+        raise ValueError("newton_schulz: CUDA tensors")
+    outs = [torch.empty(t.shape, dtype=out_dtype, device=t.device) for t in mats]
+    jobs = []
+    for t, o in zip(mats, outs):
+        r, c = t.shape[-2], t.shape[-1]
+        if t.numel() == 0:
+            continue
+        for i in range(t.numel() // (r * c)):
+            jobs.append((t.data_ptr() + i * r * c * t.element_size(), o.data_ptr() + i * r * c * o.element_size(), r, c))
+    lib = _lib.hip()
+    with _on_device_of(first):
+        for k in range(0, len(jobs), _NS_MAXMAT):
+            part = jobs[k:k + _NS_MAXMAT]
+            rows, cols = _ints([j[2] for j in part]), _ints([j[3] for j in part])
+            ws = torch.empty(lib.dtp_ns_workspace(len(part), rows, cols), dtype=torch.uint8, device=first.device)
+            check(lib.dtp_newton_schulz(len(part), _ptrs([j[0] for j in part]), _ptrs([j[1] for j in part]), rows, cols,
+                                        NS_DTYPES[first.dtype], NS_DTYPES[out_dtype], int(steps), cf, sc, float(eps),
+                                        ptr(ws), ws.numel(), stream()), "newton_schulz")
+    return outs if many else outs[0]
+
+
+MUON_ADJUST = {"match_rms_adamw": lambda r, c: 0.2 * _math.sqrt(max(r, c)),
+               "original": lambda r, c: _math.sqrt(max(1.0, r / c))}
+
+
+def muon_step(params, grads, bufs, lps, lr, momentum=0.95, nesterov=True, weight_decay=0.1, steps=5, coeffs=NS_COEFFS,
+              eps=1e-7, adjust_lr="match_rms_adamw", grad_scale=1.0):
+    """One Muon step over lists of matrices, in place:
+
+        d = grad * grad_scale;  buf = momentum * buf + (1 - momentum) * d
+        u = (1 - momentum) * d + momentum * buf  if nesterov else  buf
+        w = w * (1 - lr * weight_decay) - lr * s(shape) * newton_schulz(u);   lp = bf16(w)
+
+    s = 0.2 sqrt(max(rows, cols)) ("match_rms_adamw": updates as large as AdamW's, its lr and weight decay carry
+    over) or sqrt(max(1, rows / cols)) ("original").  params, bufs: f32; grads: f32 or bf16; lps: bf16 or None for
+    each; all contiguous [rows, cols], no tensor twice."""
+    cf, sc = _ns_check_schedule(steps, coeffs, eps)
+    if adjust_lr not in MUON_ADJUST:
+        raise ValueError("muon_step: adjust_lr must be one of %s, got %r" % (sorted(MUON_ADJUST), adjust_lr))
+    if not 0.0 <= momentum < 1.0:
+        raise ValueError("muon_step: momentum must be in [0, 1), got %r" % (momentum,))
+    n = len(params)
+    if not (len(grads) == len(bufs) == len(lps) == n):
+        raise ValueError("muon_step: %d params, %d grads, %d bufs, %d lps" % (n, len(grads), len(bufs), len(lps)))
+    if n == 0:
+        return
+    written = set()
+    for p, g, m, lp in zip(params, grads, bufs, lps):
+        if p.dim() != 2 or p.dtype != torch.float32 or m.dtype != torch.float32 or g.dtype != grads[0].dtype \
+                or g.dtype not in (torch.float32, BF16) or (lp is not None and lp.dtype != BF16):
+            raise ValueError("muon_step: f32 [rows, cols] params and bufs, f32 or bf16 grads, bf16 lps")
+        for t in (p, g, m) + ((lp,) if lp is not None else ()):
+            if t.shape != p.shape or t.device != params[0].device or not t.is_contiguous():
+                raise ValueError("muon_step: params, grads, bufs and lps must agree in shape and device and be contiguous")
+        for t in (p, m) + ((lp,) if lp is not None else ()):
+            if t.numel() and t.data_ptr() in written:
+                raise ValueError("muon_step: a tensor that is written appears twice")
+            written.add(t.data_ptr())
+        if g.numel() and g.data_ptr() in (p.data_ptr(), m.data_ptr()):
+            raise ValueError("muon_step: a gradient shares its memory with what is written")
+        _ns_check_sides(p.shape[0], p.shape[1])
+    if not params[0].is_cuda:
+        raise ValueError("muon_step: CUDA tensors")
+    jobs = [j for j in zip(params, grads, bufs, lps) if j[0].numel()]
+    lib = _lib.hip()
+    scale = MUON_ADJUST[adjust_lr]
+    with _on_device_of(params[0]):
+        for k in range(0, len(jobs), _NS_MAXMAT):
+            part = jobs[k:k + _NS_MAXMAT]
+            shapes = [j[0].shape for j in part]
+            rows, cols = _ints([s[0] for s in shapes]), _ints([s[1] for s in shapes])
+            ws = torch.empty(lib.dtp_ns_workspace(len(part), rows, cols), dtype=torch.uint8, device=params[0].device)
+            check(lib.dtp_muon_step(len(part), _ptrs([j[0].data_ptr() for j in part]), _ptrs([j[1].data_ptr() for j in part]),
+                                    _ptrs([j[2].data_ptr() for j in part]),
+                                    _ptrs([0 if j[3] is None else j[3].data_ptr() for j in part]), rows, cols,
+                                    int(part[0][1].dtype == BF16), float(momentum), int(bool(nesterov)), float(grad_scale),
+                                    _floats([1.0 - lr * weight_decay] * len(part)),
+                                    _floats([lr * scale(s[0], s[1]) for s in shapes]), int(steps), cf, sc, float(eps),
+                                    ptr(ws), ws.numel(), stream()), "muon_step")

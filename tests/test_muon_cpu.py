@@ -1,0 +1,72 @@
+"""Newton-Schulz / Muon on the CPU: what the entry points refuse, and the scales of the f16 pairs."""
+import pytest
+import torch
+
+from distributed_training_pytorch_amd.ops import kernels as K
+
+F32, BF16 = torch.float32, torch.bfloat16
+Z = torch.zeros
+
+
+@pytest.mark.parametrize("call,what", [
+    (lambda: K.newton_schulz(Z(4, 4, dtype=torch.float64)), "f32, bf16 or f16"),
+    (lambda: K.newton_schulz(Z(4)), r"\[rows, cols\]"),
+    (lambda: K.newton_schulz([Z(2, 4, 4)]), r"\[rows, cols\]"),
+    (lambda: K.newton_schulz([Z(4, 4), Z(4, 4, dtype=BF16)]), "one type"),
+    (lambda: K.newton_schulz(Z(4, 8).t()), "contiguous"),
+    (lambda: K.newton_schulz(Z(4, 4), steps=0), "steps"),
+    (lambda: K.newton_schulz(Z(4, 4), steps=13), "steps"),
+    (lambda: K.newton_schulz(Z(4, 4), steps=2.5), "steps"),
+    (lambda: K.newton_schulz(Z(4, 4), coeffs=(1.0, 2.0)), "three"),
+    (lambda: K.newton_schulz(Z(4, 4), coeffs=(1.0, 2.0, float("nan"))), "three"),
+    (lambda: K.newton_schulz(Z(4, 4), coeffs=(30.0, 1.0, 1.0)), "bounded"),
+    (lambda: K.newton_schulz(Z(4, 4), eps=0.0), "eps"),
+    (lambda: K.newton_schulz(Z(4, 4), out_dtype=torch.float64), "out_dtype"),
+    (lambda: K.newton_schulz(Z(1).expand(1, 2 ** 20 + 1).contiguous()), "2\\^20"),
+    (lambda: K.newton_schulz(Z(4, 4)), "CUDA"),
+    (lambda: K.muon_step([Z(4, 4)], [Z(4, 4)], [Z(4, 4)], [], lr=0.1), "1 params"),
+    (lambda: K.muon_step([Z(4)], [Z(4)], [Z(4)], [None], lr=0.1), r"\[rows, cols\]"),
+    (lambda: K.muon_step([Z(4, 4)], [Z(4, 4)], [Z(4, 4, dtype=BF16)], [None], lr=0.1), "f32"),
+    (lambda: K.muon_step([Z(4, 4)], [Z(4, 5)], [Z(4, 4)], [None], lr=0.1), "agree in shape"),
+    (lambda: K.muon_step([Z(4, 6).t()], [Z(6, 4)], [Z(6, 4)], [None], lr=0.1), "contiguous"),
+    (lambda: K.muon_step([Z(4, 4)], [Z(4, 4)], [Z(4, 4)], [None], lr=0.1, momentum=1.0), "momentum"),
+    (lambda: K.muon_step([Z(4, 4)], [Z(4, 4)], [Z(4, 4)], [None], lr=0.1, adjust_lr="none"), "adjust_lr"),
+    (lambda: K.muon_step([Z(4, 4)], [Z(4, 4)], [Z(4, 4)], [None], lr=0.1), "CUDA"),
+])
+def test_refusals(call, what):
+    with pytest.raises(ValueError, match=what):
+        call()
+
+
+def test_muon_refuses_what_is_written_twice():
+    p, g, m = Z(4, 4), Z(4, 4), Z(4, 4)
+    with pytest.raises(ValueError, match="twice"):
+        K.muon_step([p], [g], [p], [None], lr=0.1)
+    with pytest.raises(ValueError, match="shares its memory"):
+        K.muon_step([p], [m], [m], [None], lr=0.1)
+
+
+def test_segments():
+    assert [K.ns_segments(n) for n in (1, 2, 3, 4, 5, 6, 7, 10)] == [[1], [2], [3], [2, 2], [3, 2], [3, 3], [3, 2, 2], [3, 3, 2, 2]]
+
+
+@pytest.mark.parametrize("steps", [1, 5, 8])
+@pytest.mark.parametrize("coeffs", [K.NS_COEFFS, (1.5, -0.5, 0.0), (2.0, -1.5, 0.5)])
+def test_scales_keep_every_matrix_of_the_chain_in_f16(steps, coeffs):
+    """Largest entry of every matrix (<= its spectral norm, by eigenvalue) times its scale: within f16, with room."""
+    _, sc = K._ns_plan(steps, coeffs)
+    sc = list(sc)
+    assert all(2.0 ** round(torch.tensor(s).log2().item()) == s for s in sc)
+    x = torch.linspace(0, 1, 100_001, dtype=torch.float64)
+    for length in K.ns_segments(steps):
+        assert x.abs().max() * sc.pop(0) <= 16384
+        q = torch.ones_like(x)
+        for _ in range(length):
+            sa, sp, sq = sc.pop(0), sc.pop(0), sc.pop(0)
+            lam = x * x
+            p = coeffs[0] + coeffs[1] * lam + coeffs[2] * lam * lam
+            r = lam * p
+            q, x = q * p, x * p
+            for v, s in ((lam, sa), (r, sa), (p, sp), (q, sq)):
+                assert v.abs().max() * s <= 16384
+    assert not sc
