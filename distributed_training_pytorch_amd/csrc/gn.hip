@@ -118,6 +118,283 @@ DTP_DEVINL float pivot_of(const typename Pack<T, VEC>::word* xn, int group, int 
 }
 
 // ---------------------------------------------------------------------------------------------------------
+// Images whose groups fit a workgroup's registers: x is read once and y written once (backward: x and dy read once).
+// A workgroup owns a slab of whole groups of one image: HW rows of TX vectors.  Threads stand in R = NT / TX rows of TX
+// columns, a thread keeps its column and at most KV of its rows.
+struct GnSlab {
+  int SG, slabs;             // groups of a slab, slabs of an image
+};
+
+// Sums over the threads of a column, from lanes of one wave first where TX is a power of two up to 32: afterwards
+// `rows` rows of sums are to be added, and this thread has one of them if the result is >= 0.
+DTP_DEVINL int column_rows(int TX, int NT, int ty, int R, int& rows) {
+  const int lane = threadIdx.x & 63;
+  if ((TX & (TX - 1)) == 0 && TX <= 32) {
+    rows = NT >> 6;
+    return lane < TX ? (int)(threadIdx.x >> 6) : -1;
+  }
+  rows = R;
+  return ty < R ? ty : -1;
+}
+template <int CTRL> DTP_DEVINL float add_turned(float v) {       // v + v of the lane that many places on in its row of 16
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+DTP_DEVINL float column_sum(float v, int TX) {       // over the lanes l, l + TX, ... of the wave
+  if ((TX & (TX - 1)) != 0 || TX > 32) return v;
+  if (TX <= 1) v = add_turned<0x121>(v);             // row_ror:1, 2, 4, 8
+  if (TX <= 2) v = add_turned<0x122>(v);
+  if (TX <= 4) v = add_turned<0x124>(v);
+  if (TX <= 8) v = add_turned<0x128>(v);
+  if (TX <= 16) v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+// groups (within a slab) of VEC neighbouring channels from c
+template <int VEC> DTP_DEVINL void groups_of(int c, int cpg, int* g) {
+  int q = c / cpg, left = cpg - (c - q * cpg);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    g[e] = q;
+    if (--left == 0) { ++q; left = cpg; }
+  }
+}
+
+template <class T, int VEC, int NT, int KV>
+__global__ __launch_bounds__(NT) void gn_slab_fwd_kernel(const void* __restrict__ x_, const float* __restrict__ gamma,
+                                                         const float* __restrict__ beta, void* __restrict__ y_,
+                                                         float* __restrict__ stats, const GnShape s, const GnSlab sl,
+                                                         const float eps, const int act) {
+  typedef typename Pack<T, VEC>::word word;
+  extern __shared__ float sm[];                     // [2][rows][units of a row], then [SG][2] mean, rstd
+  const int block = xcd_remap(blockIdx.x, gridDim.x);
+  const int n = block / sl.slabs, slab = block - n * sl.slabs;
+  const int g0 = slab * sl.SG, ng = min(sl.SG, s.G - g0);
+  const int TX = ng * s.cpg / VEC, R = NT / TX;
+  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+  const int c0 = g0 * s.cpg + tx * VEC;             // first channel of this thread
+  const size_t base = (size_t)n * s.HW * s.CV;
+  const word* xn = (const word*)x_ + base + c0 / VEC;
+  word w[KV];
+#pragma unroll
+  for (int i = 0; i < KV; ++i) {
+    const int r = ty + i * R;
+    if (ty < R && r < s.HW) w[i] = xn[(size_t)r * s.CV];
+  }
+  float p[VEC], a0[VEC], a1[VEC];
+  int gl[VEC];                                      // group within the slab
+  groups_of<VEC>(tx * VEC, s.cpg, gl);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    p[e] = pivot_of<T, VEC>((const word*)x_ + base, g0 + gl[e], s.cpg);
+    a0[e] = a1[e] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < KV; ++i) {
+    const int r = ty + i * R;
+    if (ty < R && r < s.HW) {
+      float f[VEC];
+      Pack<T, VEC>::unpack(w[i], f);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float d = f[e] - p[e];
+        a0[e] += d;
+        a1[e] = fmaf(d, d, a1[e]);
+      }
+    }
+  }
+  // neighbouring channels of one group and thread are one unit of u = gcd(cpg, VEC)
+  int u = 1;
+  if (VEC > 1 && s.cpg % 2 == 0) {
+    u = 2;
+#pragma unroll
+    for (int e = 0; e + 1 < VEC; e += 2) { a0[e] += a0[e + 1]; a1[e] += a1[e + 1]; }
+    if (VEC > 2 && s.cpg % 4 == 0) {
+      u = 4;
+#pragma unroll
+      for (int e = 0; e + 2 < VEC; e += 4) { a0[e] += a0[e + 2]; a1[e] += a1[e + 2]; }
+      if (VEC > 4 && s.cpg % 8 == 0) {
+        u = 8;
+        a0[0] += a0[VEC / 2];
+        a1[0] += a1[VEC / 2];
+      }
+    }
+  }
+  const int nu = VEC / u, m = s.cpg / u, row = TX * nu;
+  int rows;
+  const int mine = column_rows(TX, NT, ty, R, rows);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    if (e % u == 0) {
+      const float b0 = column_sum(a0[e], TX), b1 = column_sum(a1[e], TX);
+      if (mine >= 0) {
+        sm[mine * row + tx * nu + e / u] = b0;
+        sm[(rows + mine) * row + tx * nu + e / u] = b1;
+      }
+    }
+  }
+  __syncthreads();
+  float* ms = sm + 2 * rows * row;
+  const int lane = threadIdx.x & 63;
+  for (int g = threadIdx.x >> 6; g < ng; g += NT / 64) {
+    float b0 = 0.f, b1 = 0.f;
+    for (int i = lane; i < rows * m; i += 64) {
+      const int r = i / m, j = r * row + g * m + i - r * m;
+      b0 += sm[j];
+      b1 += sm[rows * row + j];
+    }
+    b0 = wave_reduce_sum(b0);
+    b1 = wave_reduce_sum(b1);
+    if (lane == 0) {
+      const double pv = (double)pivot_of<T, VEC>((const word*)x_ + base, g0 + g, s.cpg), mm = (double)s.HW * s.cpg;
+      const double d = (double)b0 / mm;
+      double var = (double)b1 / mm - d * d;
+      if (var < 0.0) var = 0.0;
+      const float mean = (float)(pv + d), rstd = (float)(1.0 / sqrt(var + (double)eps));
+      ms[2 * g] = mean;
+      ms[2 * g + 1] = rstd;
+      float* o = stats + ((size_t)n * s.G + g0 + g) * 2;
+      o[0] = mean;
+      o[1] = rstd;
+    }
+  }
+  __syncthreads();
+  float mu[VEC], rs[VEC], ga[VEC], be[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    mu[e] = ms[2 * gl[e]];
+    rs[e] = ms[2 * gl[e] + 1];
+    ga[e] = gamma[c0 + e];
+    be[e] = beta[c0 + e];
+  }
+  word* yn = (word*)y_ + base + c0 / VEC;
+#pragma unroll
+  for (int i = 0; i < KV; ++i) {
+    const int r = ty + i * R;
+    if (ty < R && r < s.HW) {
+      float f[VEC], o[VEC];
+      Pack<T, VEC>::unpack(w[i], f);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[e] = act_fwd<T>(fmaf((f[e] - mu[e]) * rs[e], ga[e], be[e]), act);
+      yn[(size_t)r * s.CV] = Pack<T, VEC>::pack(o);
+    }
+  }
+}
+
+// sums: per-channel (sum dz, sum dz*xhat) of every image, [N][2][C], for gn_dparam_kernel
+template <class T, int VEC, int NT, int KV>
+__global__ __launch_bounds__(NT) void gn_slab_bwd_kernel(const void* __restrict__ x_, const void* __restrict__ dy_,
+                                                         const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                         const float* __restrict__ stats, void* __restrict__ dx_,
+                                                         float* __restrict__ sums, const GnShape s, const GnSlab sl,
+                                                         const int act) {
+  typedef typename Pack<T, VEC>::word word;
+  extern __shared__ float sm[];                     // [2][rows][channels], [2][channels], [SG][2]
+  const int block = xcd_remap(blockIdx.x, gridDim.x);
+  const int n = block / sl.slabs, slab = block - n * sl.slabs;
+  const int g0 = slab * sl.SG, ng = min(sl.SG, s.G - g0);
+  const int SC = ng * s.cpg, TX = SC / VEC, R = NT / TX;
+  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+  const int c0 = g0 * s.cpg + tx * VEC;
+  const size_t base = (size_t)n * s.HW * s.CV + c0 / VEC;
+  const word *xn = (const word*)x_ + base, *dn = (const word*)dy_ + base;
+  word wx[KV], wd[KV];
+#pragma unroll
+  for (int i = 0; i < KV; ++i) {
+    const int r = ty + i * R;
+    if (ty < R && r < s.HW) {
+      wx[i] = xn[(size_t)r * s.CV];
+      wd[i] = dn[(size_t)r * s.CV];
+    }
+  }
+  float mu[VEC], rs[VEC], ga[VEC], be[VEC], a0[VEC], a1[VEC];
+  int gl[VEC];
+  groups_of<VEC>(tx * VEC, s.cpg, gl);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const float* st = stats + ((size_t)n * s.G + g0 + gl[e]) * 2;
+    mu[e] = st[0];
+    rs[e] = st[1];
+    ga[e] = gamma[c0 + e];
+    be[e] = beta[c0 + e];
+    a0[e] = a1[e] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < KV; ++i) {
+    const int r = ty + i * R;
+    if (ty < R && r < s.HW) {
+      float f[VEC], d[VEC];
+      Pack<T, VEC>::unpack(wx[i], f);
+      Pack<T, VEC>::unpack(wd[i], d);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float xh = (f[e] - mu[e]) * rs[e];
+        const float dz = act_bwd<T>(fmaf(xh, ga[e], be[e]), d[e], act);
+        a0[e] += dz;
+        a1[e] = fmaf(dz, xh, a1[e]);
+      }
+    }
+  }
+  int rows;
+  const int mine = column_rows(TX, NT, ty, R, rows);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const float b0 = column_sum(a0[e], TX), b1 = column_sum(a1[e], TX);
+    if (mine >= 0) {
+      sm[mine * SC + tx * VEC + e] = b0;
+      sm[(rows + mine) * SC + tx * VEC + e] = b1;
+    }
+  }
+  __syncthreads();
+  float *chs = sm + 2 * rows * SC, *ms = chs + 2 * SC;
+  for (int i = threadIdx.x; i < 2 * SC; i += NT) {
+    const int which = i >= SC, c = i - which * SC;
+    float t = 0.f;
+    for (int r = 0; r < rows; ++r) t += sm[(which * rows + r) * SC + c];
+    sums[((size_t)n * 2 + which) * s.C + g0 * s.cpg + c] = t;
+    chs[i] = t * gamma[g0 * s.cpg + c];
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63;
+  const float inv = 1.f / ((float)s.HW * (float)s.cpg);
+  for (int g = threadIdx.x >> 6; g < ng; g += NT / 64) {
+    float b0 = 0.f, b1 = 0.f;
+    for (int c = lane; c < s.cpg; c += 64) {
+      b0 += chs[g * s.cpg + c];
+      b1 += chs[SC + g * s.cpg + c];
+    }
+    b0 = wave_reduce_sum(b0);
+    b1 = wave_reduce_sum(b1);
+    if (lane == 0) {
+      ms[2 * g] = b0 * inv;
+      ms[2 * g + 1] = b1 * inv;
+    }
+  }
+  __syncthreads();
+  float m1[VEC], m2[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    m1[e] = ms[2 * gl[e]];
+    m2[e] = ms[2 * gl[e] + 1];
+  }
+  word* on = (word*)dx_ + base;
+#pragma unroll
+  for (int i = 0; i < KV; ++i) {
+    const int r = ty + i * R;
+    if (ty < R && r < s.HW) {
+      float f[VEC], d[VEC], o[VEC];
+      Pack<T, VEC>::unpack(wx[i], f);
+      Pack<T, VEC>::unpack(wd[i], d);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float xh = (f[e] - mu[e]) * rs[e];
+        const float dz = act_bwd<T>(fmaf(xh, ga[e], be[e]), d[e], act);
+        o[e] = rs[e] * (fmaf(ga[e], dz, -m1[e]) - xh * m2[e]);
+      }
+      on[(size_t)r * s.CV] = Pack<T, VEC>::pack(o);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------
 // Any size: partial sums over pieces of an image, a fold, and a second pass over the data.
 // A block's threads stand in rows of min(C / VEC, 256) columns; a thread keeps its column, so its channels'
 // parameters stay in registers.
@@ -247,22 +524,44 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const void* __restrict__ 
   }
 }
 
-// Backward: per image, fold the pieces to per-channel sums [N][2][C] and per-group (m1, m2) [N][G][2]
-__global__ __launch_bounds__(256) void gn_bwd_fold_kernel(const float* __restrict__ partial,
-                                                          const float* __restrict__ gamma, float* __restrict__ sums,
-                                                          float* __restrict__ coef, const GnShape s) {
+// Backward: per image, fold the pieces to per-channel sums [N][2][C] and per-group (m1, m2) [N][G][2].  A thread adds
+// every `parts`-th piece of one value, eight loads under way (one thread a value, one load at a time: 20 us for 64 images
+// of 56x56x256 in 32 pieces).
+constexpr int GN_FOLD = 1024;
+__global__ __launch_bounds__(GN_FOLD) void gn_bwd_fold_kernel(const float* __restrict__ partial,
+                                                              const float* __restrict__ gamma, float* __restrict__ sums,
+                                                              float* __restrict__ coef, const GnShape s) {
   extern __shared__ float sm[];                     // [2][C]
-  const int n = blockIdx.x;
-  for (int i = threadIdx.x; i < 2 * s.C; i += 256) {
+  __shared__ double part[GN_FOLD];
+  const int n = blockIdx.x, W = 2 * s.C;
+  const float* pn = partial + (size_t)n * s.chunks * W;
+  const int parts = W >= GN_FOLD ? 1 : GN_FOLD / W, cols = min(W, GN_FOLD);
+  for (int i0 = 0; i0 < W; i0 += cols) {
+    const int i = i0 + threadIdx.x % cols, q = threadIdx.x / cols;
     double t = 0.0;
-    for (int k = 0; k < s.chunks; ++k) t += (double)partial[((size_t)n * s.chunks + k) * 2 * s.C + i];
-    sums[(size_t)n * 2 * s.C + i] = (float)t;
-    sm[i] = (float)t * gamma[i >= s.C ? i - s.C : i];
+    if (q < parts && i < W) {
+      int k = q;
+      for (; k + 7 * parts < s.chunks; k += 8 * parts) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = pn[(size_t)(k + e * parts) * W + i];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t += (double)v[e];
+      }
+      for (; k < s.chunks; k += parts) t += (double)pn[(size_t)k * W + i];
+    }
+    part[threadIdx.x] = t;
+    __syncthreads();
+    if (q == 0 && i < W) {
+      for (int k = 1; k < parts; ++k) t += part[k * cols + threadIdx.x];
+      sums[(size_t)n * W + i] = (float)t;
+      sm[i] = (float)t * gamma[i >= s.C ? i - s.C : i];
+    }
+    __syncthreads();
   }
-  __syncthreads();
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const float inv = 1.f / ((float)s.HW * (float)s.cpg);
-  for (int g = wave; g < s.G; g += 4) {
+  for (int g = wave; g < s.G; g += GN_FOLD / 64) {
     float u = 0.f, v = 0.f;
     for (int c = lane; c < s.cpg; c += 64) {
       u += sm[g * s.cpg + c];
@@ -384,6 +683,50 @@ int gn_vec(int C, int elem) {
   return v;
 }
 
+int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+// LDS of a slab kernel (a slab may be the image's last, with fewer groups: any number of columns has its place)
+size_t slab_lds(const GnShape& s, int vec, int sg, int nt, int bwd) {
+  const size_t row = (size_t)2 * nt * (bwd ? vec : vec / gcd(s.cpg, vec));
+  return (row + (bwd ? (size_t)2 * sg * s.cpg : 0) + 2 * (size_t)sg) * sizeof(float);
+}
+
+// Whether a slab of `sg` groups fits (columns, rows a thread, 64 KB of LDS): 0 no, else the threads
+int slab_fits(const GnShape& s, int vec, int sg, int bwd) {
+  static const int nt[3] = {256, 512, 1024}, kv[2][3] = {{8, 16, 16}, {8, 16, 0}};
+  const long tx = (long)sg * s.cpg / vec;
+  for (int v = 0; v < 3; ++v)
+    if (kv[bwd][v] && tx <= nt[v] && (s.HW + nt[v] / tx - 1) / (nt[v] / tx) <= kv[bwd][v] &&
+        slab_lds(s, vec, sg, nt[v], bwd) <= 65536)
+      return nt[v];
+  return 0;
+}
+
+// Groups of a slab; 0: none fits, or its rows are so short (64 bytes, 32, 16) that the loads cost more than a second
+// pass.  Rows should be whole cache lines, but the workgroups 512 at least.  Measured (us, slab / two passes; bf16, 32
+// groups): rows of 64 bytes and more always pay (forward 64x56x56x256 41 / 67, backward 64x28x28x512 55 / 88); of 32:
+// forward 4x28x28x512 9 / 19, backward the same 18.5 / 45, but backward 64x56x56x256 146 / 118; of 16: 4x56x56x256
+// forward 12 / 19, backward 23 / 44, but forward 64x112x112x128 182 / 127.
+int slab_groups(const GnShape& s, int vec, int elem, int bwd, int& threads) {
+  const int step = vec / gcd(s.cpg, vec);            // groups that make whole vectors
+  const long total = (long)s.N * s.HW * s.C * elem;
+  int best = 0;
+  for (int sg = step; sg <= s.G; sg += step) {
+    const int f = slab_fits(s, vec, sg, bwd);
+    if (!f) break;
+    const long blocks = (long)s.N * ((s.G + sg - 1) / sg), bytes = (long)sg * s.cpg * elem;
+    if (best && (blocks < 512 || bytes > 128)) break;
+    best = sg;
+    threads = f;
+    if (bytes >= 128) break;
+  }
+  if (!best || best == s.G) return best;
+  const long bytes = (long)best * s.cpg * elem;
+  if (bytes < 32) return total <= (8L << 20) ? best : 0;
+  if (bytes < 64 && bwd) return total <= (32L << 20) ? best : 0;
+  return best;
+}
+
 size_t partial_floats(const GnShape& s, int bwd) {
   return bwd ? (size_t)s.N * s.chunks * 2 * s.C : (size_t)s.N * s.chunks * s.G * 2;
 }
@@ -391,6 +734,18 @@ size_t partial_floats(const GnShape& s, int bwd) {
 template <class T, int VEC>
 int gn_run_fwd(const void* x, const float* gamma, const float* beta, void* y, float* stats, float* ws, size_t ws_floats,
                const GnShape& s, float eps, int act, hipStream_t st) {
+  int NT = 0;
+  GnSlab sl;
+  sl.SG = slab_groups(s, VEC, T::size, 0, NT);
+  if (sl.SG) {
+    sl.slabs = (s.G + sl.SG - 1) / sl.SG;
+    const size_t lds = slab_lds(s, VEC, sl.SG, NT, 0);
+    const dim3 g((unsigned)(s.N * sl.slabs));
+    if (NT == 256) hipLaunchKernelGGL((gn_slab_fwd_kernel<T, VEC, 256, 8>), g, dim3(256), lds, st, x, gamma, beta, y, stats, s, sl, eps, act);
+    else if (NT == 512) hipLaunchKernelGGL((gn_slab_fwd_kernel<T, VEC, 512, 16>), g, dim3(512), lds, st, x, gamma, beta, y, stats, s, sl, eps, act);
+    else hipLaunchKernelGGL((gn_slab_fwd_kernel<T, VEC, 1024, 16>), g, dim3(1024), lds, st, x, gamma, beta, y, stats, s, sl, eps, act);
+    return DTP_CHECK_LAUNCH();
+  }
   if (ws_floats < partial_floats(s, 0)) return -12;
   const size_t lds = (size_t)(2 * s.C + 2 * GN_T * VEC) * sizeof(float);
   const dim3 grid(s.N * s.chunks);
@@ -405,12 +760,26 @@ int gn_run_bwd(const void* x, const void* dy, const float* gamma, const float* b
                void* dgamma, void* dbeta, int out_fp32, float beta_g, float beta_b, float* ws, size_t ws_floats,
                const GnShape& s, int act, hipStream_t st) {
   const size_t np = partial_floats(s, 1), ns = (size_t)s.N * 2 * s.C, nc = (size_t)s.N * s.G * 2;
+  if (ws_floats < ns) return -12;
+  float *sums = ws, *coef = sums + ns, *partial = coef + nc;
+  int NT = 0;
+  GnSlab sl;
+  sl.SG = slab_groups(s, VEC, T::size, 1, NT);
+  if (sl.SG) {
+    sl.slabs = (s.G + sl.SG - 1) / sl.SG;
+    const size_t slds = slab_lds(s, VEC, sl.SG, NT, 1);
+    const dim3 g((unsigned)(s.N * sl.slabs));
+    if (NT == 256) hipLaunchKernelGGL((gn_slab_bwd_kernel<T, VEC, 256, 8>), g, dim3(256), slds, st, x, dy, gamma, beta, stats, dx, sums, s, sl, act);
+    else hipLaunchKernelGGL((gn_slab_bwd_kernel<T, VEC, 512, 16>), g, dim3(512), slds, st, x, dy, gamma, beta, stats, dx, sums, s, sl, act);
+    hipLaunchKernelGGL(gn_dparam_kernel, dim3((s.C + 15) / 16), dim3(256), 0, st, sums, s.N, s.C, dgamma, dbeta, out_fp32,
+                       beta_g, beta_b);
+    return DTP_CHECK_LAUNCH();
+  }
   if (ws_floats < np + ns + nc) return -12;
-  float *sums = ws + np, *coef = sums + ns;
   const size_t lds = (size_t)(2 * s.C + 2 * GN_T * VEC) * sizeof(float);
   const dim3 grid(s.N * s.chunks);
-  hipLaunchKernelGGL((gn_partial_kernel<T, VEC, 1>), grid, dim3(GN_T), lds, st, x, dy, gamma, beta, stats, ws, s, act);
-  hipLaunchKernelGGL(gn_bwd_fold_kernel, dim3(s.N), dim3(256), (size_t)2 * s.C * sizeof(float), st, ws, gamma, sums, coef, s);
+  hipLaunchKernelGGL((gn_partial_kernel<T, VEC, 1>), grid, dim3(GN_T), lds, st, x, dy, gamma, beta, stats, partial, s, act);
+  hipLaunchKernelGGL(gn_bwd_fold_kernel, dim3(s.N), dim3(GN_FOLD), (size_t)2 * s.C * sizeof(float), st, partial, gamma, sums, coef, s);
   hipLaunchKernelGGL((gn_apply_kernel<T, VEC, 1>), grid, dim3(GN_T), 0, st, x, dy, gamma, beta, stats, coef, dx, s, act);
   hipLaunchKernelGGL(gn_dparam_kernel, dim3((s.C + 15) / 16), dim3(256), 0, st, sums, s.N, s.C, dgamma, dbeta, out_fp32,
                      beta_g, beta_b);
@@ -438,12 +807,15 @@ int gn_run_bwd(const void* x, const void* dy, const float* gamma, const float* b
     return FN<tag_bf16, 1>(__VA_ARGS__);                          \
   } while (0)
 
-// Floats of scratch that dtp_gn_fwd (bwd = 0) / dtp_gn_bwd (bwd = 1) need; 0: shape refused.
+// Floats of scratch that dtp_gn_fwd (bwd = 0) / dtp_gn_bwd (bwd = 1) need; (size_t)-1: shape refused.
 extern "C" size_t dtp_gn_workspace(int N, int HW, int C, int G, int dtype, int bwd) {
-  if (!gn_ok(N, HW, C, G, dtype, 0)) return 0;
-  const int elem = dtype == 2 ? 4 : 2;
-  const GnShape s = shape_of(N, HW, C, G, gn_vec(C, elem), elem);
-  return partial_floats(s, bwd) + (bwd ? (size_t)N * 2 * C + (size_t)N * G * 2 : 0);
+  if (!gn_ok(N, HW, C, G, dtype, 0)) return (size_t)-1;
+  const int elem = dtype == 2 ? 4 : 2, vec = gn_vec(C, elem);
+  const GnShape s = shape_of(N, HW, C, G, vec, elem);
+  int nt;
+  const size_t sums = bwd ? (size_t)N * 2 * C : 0;
+  if (slab_groups(s, vec, elem, bwd, nt)) return sums;
+  return sums + partial_floats(s, bwd) + (bwd ? (size_t)N * G * 2 : 0);
 }
 
 // x, y: [N][HW][C] (dtype 0 bf16, 1 f16, 2 f32), 16-byte aligned; gamma, beta: f32 [C]; stats: f32 [N][G][2] (mean, rstd)

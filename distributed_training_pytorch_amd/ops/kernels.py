@@ -993,6 +993,14 @@ def _gn_check(x, groups, act, *vecs):
     return N, HW, C, G
 
 
+@_functools.lru_cache(maxsize=256)
+def _gn_workspace(N, HW, C, G, dt, bwd):
+    n = _lib.hip().dtp_gn_workspace(N, HW, C, G, dt, bwd)
+    if n == (1 << (8 * _ctypes.sizeof(_ctypes.c_size_t))) - 1:
+        raise RuntimeError("group norm: the native library refuses [%d, %d, %d] in %d groups" % (N, HW, C, G))
+    return n
+
+
 def gn_fwd(x, gamma, beta, groups, eps=1e-5, act="relu"):
     """y = act(group_norm(x)) over channels-last x [N, ..., C] (bf16, f16 or f32, contiguous): per image and
     group of C / groups neighbouring channels, mean and variance over all positions; gamma / beta f32 [C];
@@ -1008,8 +1016,9 @@ def gn_fwd(x, gamma, beta, groups, eps=1e-5, act="relu"):
     with _on_device_of(x):
         # scratch of this call alone (the caching allocator's, so a captured graph keeps its own): calls on two
         # streams, or two graphs, share nothing
-        ws = torch.empty(lib.dtp_gn_workspace(N, HW, C, G, dt, 0), dtype=torch.float32, device=x.device)
-        check(lib.dtp_gn_fwd(ptr(x), ptr(gamma), ptr(beta), ptr(y), ptr(stats), ptr(ws), ws.numel(), N, HW, C, G, dt,
+        n = _gn_workspace(N, HW, C, G, dt, 0)
+        ws = torch.empty(n, dtype=torch.float32, device=x.device) if n else None
+        check(lib.dtp_gn_fwd(ptr(x), ptr(gamma), ptr(beta), ptr(y), ptr(stats), ptr(ws), n, N, HW, C, G, dt,
                              GN_ACTS[act], float(eps), stream()), "gn_fwd")
     return y, stats
 
@@ -1037,7 +1046,7 @@ def gn_bwd(x, dy, gamma, beta, stats, groups, dgamma, dbeta, act="relu", beta_g=
     dt = GN_DTYPES[x.dtype]
     lib = _lib.hip()
     with _on_device_of(x):
-        ws = torch.empty(lib.dtp_gn_workspace(N, HW, C, G, dt, 1), dtype=torch.float32, device=x.device)
+        ws = torch.empty(_gn_workspace(N, HW, C, G, dt, 1), dtype=torch.float32, device=x.device)
         check(lib.dtp_gn_bwd(ptr(x), ptr(dy), ptr(gamma), ptr(beta), ptr(stats), ptr(dx), ptr(dgamma), ptr(dbeta),
                              int(dgamma.dtype == torch.float32), float(beta_g), float(beta_b), ptr(ws), ws.numel(), N, HW,
                              C, G, dt, GN_ACTS[act], stream()), "gn_bwd")
