@@ -67,6 +67,8 @@ def parse_args(argv=None):
                          "host ring, H2D copy on the copy stream inside the timed region, normalisation fused "
                          "into the first convolution (the reference's pinned loader + per-step H2D, main.py:16)")
     ap.add_argument("--batch-norm", action="store_true", help="VGG16-BN (BASELINE.json config 5)")
+    ap.add_argument("--group-norm", type=int, default=0, metavar="GROUPS", help="VGG16-GN")
+    ap.add_argument("--optimizer", default="sgd", choices=["sgd", "muon"])
     ap.add_argument("--fp8-classifier", action="store_true", help="linear1/linear2 GEMMs in OCP e4m3 (config 5)")
     ap.add_argument("--shard-optimizer", action="store_true",
                     help="reduce-scatter + per-bucket sharded SGD + all-gather instead of all-reduce + replicated SGD")
@@ -127,6 +129,10 @@ def preflight_native(args, world):
             child.append(flag)
     if args.image_size != 224:
         child += ["--image-size", str(args.image_size)]
+    if args.group_norm:
+        child += ["--group-norm", str(args.group_norm)]
+    if args.optimizer != "sgd":
+        child += ["--optimizer", args.optimizer]
     env = {"DTP_NATIVE_INIT_TIMEOUT_S": os.environ.get("DTP_NATIVE_INIT_TIMEOUT_S", "60"),
            "DTP_PG_TIMEOUT_S": os.environ.get("DTP_PG_TIMEOUT_S", "180")}
     if mode != "force":
@@ -210,16 +216,19 @@ def main(argv=None):
     from distributed_training_pytorch_amd.data.synthetic import DeviceBatchSource
     from distributed_training_pytorch_amd.models.vgg16 import VGG16
     from distributed_training_pytorch_amd.ops.layers import SoftmaxCrossEntropy
-    from distributed_training_pytorch_amd.ops.optim import FusedSGD
+    from distributed_training_pytorch_amd.ops.optim import FusedMuon, FusedSGD
     from distributed_training_pytorch_amd.parallel.data_parallel import DataParallel
 
     torch.manual_seed(0)
     gdt = torch.bfloat16 if (args.grad_dtype == "bf16" and on_gpu) else torch.float32
     model = VGG16(3, args.classes, True, grad_dtype=gdt, batch_norm=args.batch_norm,
-                  fp8_classifier=args.fp8_classifier).to(dev)
-    opt = FusedSGD(model, lr=args.lr, momentum=0.9, weight_decay=1e-4)
+                  fp8_classifier=args.fp8_classifier, group_norm=args.group_norm).to(dev)
+    if args.optimizer == "muon":
+        opt = FusedMuon(model, lr=args.lr, weight_decay=1e-4)
+    else:
+        opt = FusedSGD(model, lr=args.lr, momentum=0.9, weight_decay=1e-4)
     crit = SoftmaxCrossEntropy()
-    per_bucket = not args.shard_optimizer and not args.no_bucket_optimizer
+    per_bucket = not args.shard_optimizer and not args.no_bucket_optimizer and args.optimizer == "sgd"
     dp = DataParallel(model, shard_optimizer=opt if args.shard_optimizer else None,
                       bucket_optimizer=opt if per_bucket else None)
     dp.train()
@@ -346,7 +355,7 @@ def main(argv=None):
         global_batch = args.batch_per_gpu * world
         value = global_batch * args.steps / dt
         info = getattr(tr, "info", None) or {}
-        plain = not (args.batch_norm or args.fp8_classifier)
+        plain = not (args.batch_norm or args.fp8_classifier or args.group_norm) and args.optimizer == "sgd"
         sys.stdout.flush()
         if real_stdout is not None:
             os.dup2(real_stdout, 1)
@@ -377,11 +386,12 @@ def main(argv=None):
             "rccl_env_applied_by_bench": applied_env,
             "preflight": pre,       # N > 1: rehearsal of the native transport in throw-away children (None: not run)
             "config": {"model": "VGG16 (%s, %d classes, %dM params)" % (
-                           "BN" if args.batch_norm else "no BN", args.classes,
+                           "BN" if args.batch_norm else "GN%d" % args.group_norm if args.group_norm else "no BN", args.classes,
                            round(sum(p.numel() for p in model.parameters()) / 1e6)),
                        "global_batch": global_batch, "image_size": args.image_size,
                        "seq_len": None, "parallelism": "dp%d" % world,
-                       "optimizer": "fused SGD momentum 0.9 wd 1e-4, fp32 master weights%s" % (
+                       "optimizer": "fused Muon wd 1e-4, fp32 master weights" if args.optimizer == "muon" else
+                       "fused SGD momentum 0.9 wd 1e-4, fp32 master weights%s" % (
                            ", sharded per bucket (reduce-scatter + all-gather)" if dp.reducer.sharded else
                            ", per bucket behind its all-reduce" if dp.reducer.fused_update else ""),
                        "grad_dtype": args.grad_dtype if on_gpu else "fp32", "grad_accum": args.grad_accum,

@@ -66,6 +66,8 @@ _SIGS = {
                               c_int, c_int, c_int, c_int, c_float, c_float, c_void_p, c_int, c_void_p],
     "dtp_bn_bwd_pool": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float,
                         c_float, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
+    "dtp_adamw_ranges": [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_float, c_float,
+                         c_float, c_float, c_float, c_float, c_float, c_float, c_void_p],
     "dtp_gn_workspace": [c_int, c_int, c_int, c_int, c_int, c_int],
     "dtp_gn_fwd": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_int, c_int, c_int, c_int, c_int,
                    c_int, c_float, c_void_p],

@@ -114,6 +114,39 @@ __global__ __launch_bounds__(256) void adamw_flat_kernel(float* __restrict__ p, 
   }
 }
 
+// AdamW over a table of arena ranges, the step number on the device: the parameters that Muon leaves to AdamW (biases,
+// normalisation affine values, the classifier's head) lie between its matrices, and a captured step must not hold the
+// step number by value.  ranges: per workgroup (first element in the arena, elements, first element in the second
+// moment's own buffer): at most 1024 elements, multiples of 4.  bias corrections 1 - beta^t = -expm1(t ln beta).
+template <bool GRAD_BF16>
+__global__ __launch_bounds__(256) void adamw_ranges_kernel(float* __restrict__ p, const void* __restrict__ g,
+                                float* __restrict__ m, float* __restrict__ v, bf16_t* __restrict__ lp,
+                                const long* __restrict__ ranges, const int* __restrict__ step, float lr, float beta1,
+                                float beta2, float log_beta1, float log_beta2, float eps, float wd, float grad_scale) {
+  const long* r = ranges + 3 * (long)blockIdx.x;
+  const long first = r[0], count = r[1], at_v = r[2];
+  const float t = (float)*step;
+  const float size = lr / -expm1f(t * log_beta1), bc2_sqrt = sqrtf(-expm1f(t * log_beta2));
+  const long i4 = threadIdx.x;
+  if (i4 * 4 >= count) return;
+  const size_t i = (size_t)first / 4 + i4;
+  const f32x4_t gg = load_grad4<GRAD_BF16>(g, i) * grad_scale;
+  f32x4_t pn = *(const f32x4_t*)(p + i * 4) * (1.f - lr * wd);
+  const f32x4_t mn = *(const f32x4_t*)(m + i * 4) * beta1 + gg * (1.f - beta1);
+  const f32x4_t vn = *(const f32x4_t*)(v + at_v + i4 * 4) * beta2 + gg * gg * (1.f - beta2);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) pn[e] -= size * mn[e] / (sqrtf(vn[e]) / bc2_sqrt + eps);
+  *(f32x4_t*)(p + i * 4) = pn;
+  *(f32x4_t*)(m + i * 4) = mn;
+  *(f32x4_t*)(v + at_v + i4 * 4) = vn;
+  if (lp) {
+    u32x2_t o;
+    o[0] = pack_bf16x2(pn[0], pn[1]);
+    o[1] = pack_bf16x2(pn[2], pn[3]);
+    *(u32x2_t*)(lp + i * 4) = o;
+  }
+}
+
 // 2 workgroups (8 waves) per CU by default; DTP_OPT_GRID_CAP overrides (A/B: 4096 = the old full-chip grid)
 static inline int grid_for(size_t work) {
   static int cap = 0;
@@ -155,5 +188,18 @@ extern "C" int dtp_adamw_flat(float* p, const void* g, int grad_bf16, float* m, 
   else
     hipLaunchKernelGGL(adamw_flat_kernel<false>, dim3(grid_for(n / 4)), dim3(256), 0, s, p, g, m, v, (bf16_t*)lp, n / 4,
                        lr, beta1, beta2, eps, wd, grad_scale, bc1, bc2_sqrt);
+  return DTP_CHECK_LAUNCH();
+}
+
+extern "C" int dtp_adamw_ranges(float* p, const void* g, int grad_bf16, float* m, float* v, void* lp, const long* ranges,
+                                int count, const int* step, float lr, float beta1, float beta2, float log_beta1,
+                                float log_beta2, float eps, float wd, float grad_scale, hipStream_t s) {
+  if (count < 1 || !(log_beta1 < 0.f) || !(log_beta2 < 0.f)) return -10;
+  if (grad_bf16)
+    hipLaunchKernelGGL(adamw_ranges_kernel<true>, dim3(count), dim3(256), 0, s, p, g, m, v, (bf16_t*)lp, ranges, step, lr,
+                       beta1, beta2, log_beta1, log_beta2, eps, wd, grad_scale);
+  else
+    hipLaunchKernelGGL(adamw_ranges_kernel<false>, dim3(count), dim3(256), 0, s, p, g, m, v, (bf16_t*)lp, ranges, step, lr,
+                       beta1, beta2, log_beta1, log_beta2, eps, wd, grad_scale);
   return DTP_CHECK_LAUNCH();
 }

@@ -19,8 +19,8 @@ import os
 import torch
 import torch.nn as nn
 
-from ..ops.layers import (AvgPoolFlatten, BatchNormReLU, Conv3x3, ConvFirst, Linear, MaxPool2x2, ReLUMarker,
-                          bn_relu_pool, conv_bn_relu_folded, conv_relu_pool)
+from ..ops.layers import (AvgPoolFlatten, BatchNormReLU, Conv3x3, ConvFirst, GroupNormAct, Linear, MaxPool2x2,
+                          ReLUMarker, bn_relu_pool, conv_bn_relu_folded, conv_relu_pool)
 from .fused_model import FusedModel
 
 
@@ -28,12 +28,14 @@ SELF_MASK = os.environ.get("DTP_CONV1_SELF_MASK", "1") == "1"     # A/B switch (
 
 
 class ConvBlock(nn.Module):
-    def __init__(self, in_channels, out_channels, num_layers=2, first=False, batch_norm=False):
+    def __init__(self, in_channels, out_channels, num_layers=2, first=False, batch_norm=False, group_norm=0):
         super().__init__()
+        if batch_norm and group_norm:
+            raise ValueError("ConvBlock: batch_norm or group_norm, not both")
         layers = []
         for i in range(num_layers):
             cin = in_channels if i == 0 else out_channels
-            fused_relu = not batch_norm
+            fused_relu = not (batch_norm or group_norm)
             if first and i == 0:
                 # conv1_1 masks its own incoming gradient inside its weight-gradient kernel (it
                 # recomputes the forward sign from the image), so conv1_2's data-gradient does not
@@ -55,13 +57,16 @@ class ConvBlock(nn.Module):
                 # conv -> BatchNorm -> ReLU: normalisation and ReLU are one hand-written kernel pair
                 # (csrc/bn.hip); the marker keeps the Sequential indices of a torch VGG16-BN
                 layers.append(BatchNormReLU(out_channels))
+            elif group_norm:
+                layers.append(GroupNormAct(group_norm, out_channels, act="relu"))      # csrc/gn.hip, ReLU included
             layers.append(ReLUMarker())
-        layers.append(MaxPool2x2(relu_mask=not batch_norm))
+        layers.append(MaxPool2x2(relu_mask=fused_relu))
         self.conv = nn.Sequential(*layers)
         self.batch_norm = batch_norm
+        self.group_norm = int(group_norm)
 
     def forward(self, x):
-        if x.is_cuda and not self.batch_norm:
+        if x.is_cuda and not self.batch_norm and not self.group_norm:
             # last conv + ReLU + pool as one kernel where the shapes allow it (block 1: the
             # 1.6 GB pre-pool activation at batch 256 is neither written nor re-read)
             mods = list(self.conv)
@@ -114,15 +119,17 @@ class ConvBlock(nn.Module):
 
 class VGG16(FusedModel):
     def __init__(self, in_channels=3, out_channels=1, init_weights=True, batch_norm=False,
-                 dropout=0.3, grad_dtype=torch.float32, fp8_classifier=False):
+                 dropout=0.3, grad_dtype=torch.float32, fp8_classifier=False, group_norm=0):
         super().__init__(grad_dtype=grad_dtype)
         self.fp8_classifier = bool(fp8_classifier)   # linear1/linear2 forward GEMMs in OCP e4m3
         self.batch_norm = batch_norm
-        self.backbone = nn.Sequential(ConvBlock(in_channels, 64, first=True, batch_norm=batch_norm),
-                                      ConvBlock(64, 128, batch_norm=batch_norm),
-                                      ConvBlock(128, 256, num_layers=3, batch_norm=batch_norm),
-                                      ConvBlock(256, 512, num_layers=3, batch_norm=batch_norm),
-                                      ConvBlock(512, 512, num_layers=3, batch_norm=batch_norm))
+        self.group_norm = int(group_norm)            # groups per normalisation layer; 0: none
+        norm = dict(batch_norm=batch_norm, group_norm=self.group_norm)
+        self.backbone = nn.Sequential(ConvBlock(in_channels, 64, first=True, **norm),
+                                      ConvBlock(64, 128, **norm),
+                                      ConvBlock(128, 256, num_layers=3, **norm),
+                                      ConvBlock(256, 512, num_layers=3, **norm),
+                                      ConvBlock(512, 512, num_layers=3, **norm))
         self.avgpool = AvgPoolFlatten((7, 7))
         self.linear1 = Linear(512 * 7 * 7, 4096, relu=True, drop_p=dropout, grad_premasked=True,
                               fp8=fp8_classifier)
@@ -164,6 +171,11 @@ class VGG16(FusedModel):
         x = self.linear1(x)      # + ReLU + dropout fused
         x = self.linear2(x)
         return self.finish_forward(self.linear3(x))
+
+
+def vgg16_gn(in_channels=3, out_channels=1, groups=32, **kw):
+    """VGG16 with GroupNorm + ReLU behind every convolution: for small per-GPU batches, where batch statistics are poor."""
+    return VGG16(in_channels, out_channels, group_norm=groups, **kw)
 
 
 def vgg16_bn(in_channels=3, out_channels=1, **kw):

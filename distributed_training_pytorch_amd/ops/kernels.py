@@ -1129,6 +1129,31 @@ def adamw_flat(p, g, m, v, lp, lr, beta1, beta2, eps, wd, grad_scale, step):
     check(rc, "adamw_flat")
 
 
+def adamw_range_table(spans, device):
+    """Work table of :func:`adamw_ranges`: ``spans`` = (first element in the arena, elements, first element in the
+    second moment's buffer), multiples of 4; cut into at most 1024 elements each."""
+    rows = []
+    for first, n, at in spans:
+        if first % 4 or n % 4 or at % 4 or n <= 0:
+            raise ValueError("adamw_range_table: spans must be positive multiples of 4, got %s" % ((first, n, at),))
+        for k in range(0, n, 1024):
+            rows.append((first + k, min(1024, n - k), at + k))
+    return torch.tensor(rows, dtype=torch.int64).to(device)
+
+
+def adamw_ranges(p, g, m, v, lp, table, step, lr, beta1, beta2, eps, wd, grad_scale):
+    """AdamW on the ranges of ``table`` (:func:`adamw_range_table`); ``step``: device int32 [1], the number of this
+    step (1 for the first)."""
+    if step.dtype != torch.int32 or step.numel() != 1 or table.dtype != torch.int64 or table.shape[1] != 3 \
+            or not table.is_contiguous() or not step.is_cuda or not table.is_cuda:
+        raise ValueError("adamw_ranges: step must be a device int32, table adamw_range_table's")
+    if not (0.0 < beta1 < 1.0 and 0.0 < beta2 < 1.0):
+        raise ValueError("adamw_ranges: betas must be in (0, 1), got %r, %r" % (beta1, beta2))
+    check(_lib.hip().dtp_adamw_ranges(ptr(p), ptr(g), int(g.dtype == BF16), ptr(m), ptr(v), ptr(lp), ptr(table),
+                                      table.shape[0], ptr(step), float(lr), float(beta1), float(beta2), _math.log(beta1),
+                                      _math.log(beta2), float(eps), float(wd), float(grad_scale), stream()), "adamw_ranges")
+
+
 # ------------------------------------------------------------------------------------- Muon
 NS_COEFFS = (3.4445, -4.7750, 2.0315)
 NS_DTYPES = {torch.float32: 0, BF16: 1, torch.float16: 2}

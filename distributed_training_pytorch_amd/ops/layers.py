@@ -874,6 +874,61 @@ class BatchNormReLU(FusedLayer):
         return "%d, eps=%g, momentum=%g, relu=%s" % (self.num_features, self.eps, self.momentum, self.relu)
 
 
+# =============================================================================== group norm (+ activation)
+class _GroupNormActFn(torch.autograd.Function):
+    """Group norm + activation on channels-last activations (csrc/gn.hip): the backward recomputes the activation's
+    derivative from the saved convolution output and the forward's statistics, reduces d(gamma) / d(beta) straight
+    into the gradient arena and emits the convolution's incoming gradient."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, layer):
+        arena = _arena_of(layer)
+        x = x.contiguous()
+        y, stats = K.gn_fwd(x, arena.flat_slice(arena.flat_master, weight), arena.flat_slice(arena.flat_master, bias),
+                            layer.num_groups, layer.eps, layer.act)
+        ctx.layer = layer
+        ctx.save_for_backward(x, stats, weight, bias)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        layer = ctx.layer
+        arena = _arena_of(layer)
+        x, stats, weight, bias = ctx.saved_tensors
+        dx = K.gn_bwd(x, dy.contiguous(), arena.flat_slice(arena.flat_master, weight),
+                      arena.flat_slice(arena.flat_master, bias), stats, layer.num_groups, arena.grad(weight),
+                      arena.grad(bias), act=layer.act, beta_g=arena.grad_beta(weight), beta_b=arena.grad_beta(bias))
+        arena.notify_grad_ready(bias)
+        arena.notify_grad_ready(weight)
+        return dx, None, None, None
+
+
+class GroupNormAct(FusedLayer):
+    """GroupNorm over groups of neighbouring channels of one image, with the following activation fused ("none",
+    "relu" or "silu").  Parameter names are ``nn.GroupNorm``'s (``weight, bias``).  No batch statistics: training and
+    evaluation compute the same, whatever the batch (the reference trains on four images per GPU).  GPU: the kernels
+    of csrc/gn.hip on [N, ..., C] activations; CPU: ``F.group_norm`` on [N, C, ...]."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, act="relu"):
+        super().__init__()
+        if num_groups < 1 or num_channels % num_groups:
+            raise ValueError("GroupNormAct: %d channels in %d groups" % (num_channels, num_groups))
+        if act not in K.GN_ACTS:
+            raise ValueError("GroupNormAct: act must be one of %s, got %r" % (sorted(K.GN_ACTS), act))
+        self.num_groups, self.num_channels, self.eps, self.act = int(num_groups), int(num_channels), float(eps), act
+        self.weight = nn.Parameter(torch.ones(num_channels))
+        self.bias = nn.Parameter(torch.zeros(num_channels))
+
+    def forward(self, x):
+        if not x.is_cuda:
+            y = F.group_norm(x, self.num_groups, self.weight, self.bias, self.eps)
+            return F.relu(y) if self.act == "relu" else F.silu(y) if self.act == "silu" else y
+        return _GroupNormActFn.apply(x, self.weight, self.bias, self)
+
+    def extra_repr(self):
+        return "%d, %d, eps=%g, act=%s" % (self.num_groups, self.num_channels, self.eps, self.act)
+
+
 def conv_bn_relu_folded(conv, bn, x, pool=False):
     """Inference: ``relu(bn(conv(x)))`` as ONE convolution kernel — the eval-mode scale is folded
     into the bf16 filter copy and scale/shift into the bias (cached until the weights or the

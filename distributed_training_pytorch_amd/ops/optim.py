@@ -10,9 +10,14 @@ momentum=0.9, weight_decay=1e-4)`` and ``:88`` calls ``optimizer.step()`` (torch
 SGD's schema; ``exp_avg``/``exp_avg_sq``/``step`` — torch AdamW's) are views of
 flat state buffers and are serialised as standalone contiguous tensors.
 
+``FusedMuon`` has no counterpart in the reference: weight matrices move along the orthogonalised momentum
+(``csrc/muon.hip``), everything else by AdamW.
+
 GPU: ``csrc/optim.hip`` (fp32 master update + bf16 working-copy emission fused).  CPU: the same
 update rule on the flat buffers with a handful of torch ops (tested equal to torch.optim).
 """
+import math
+
 import torch
 
 from . import kernels as K
@@ -229,3 +234,147 @@ class FusedAdamW(_FusedBase):
             a.lp_written_by_optimizer()
         self._steps += 1
         return loss
+
+
+def _newton_schulz_cpu(x, steps, coeffs, eps):
+    a, b, c = coeffs
+    tall = x.shape[0] > x.shape[1]
+    x = x.t() if tall else x
+    x = x / (x.double().norm().float() + eps)
+    for _ in range(steps):
+        s = x @ x.t()
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return x.t() if tall else x
+
+
+class FusedMuon(_FusedBase):
+    """Muon on the flat arena: every weight matrix (a convolution's filters are one, [out channels, kh * kw * in
+    channels]) moves along its Nesterov momentum, orthogonalised by Newton-Schulz iterations:
+
+        buf = momentum * buf + (1 - momentum) * grad;   u = (1 - momentum) * grad + momentum * buf
+        w = w * (1 - lr * weight_decay) - lr * s(shape) * newton_schulz(u)
+
+    s(shape) = 0.2 sqrt(max(rows, cols)) (``adjust_lr="match_rms_adamw"``) or sqrt(max(1, rows / cols))
+    ("original").  Parameters that are no matrices (biases, normalisation), and the last matrix (the classifier's head),
+    are updated by AdamW with the same lr and weight decay; ``use_muon(name, parameter) -> bool`` chooses otherwise (for
+    parameters of two dimensions and more).  State per parameter: ``momentum_buffer`` (AdamW's first moment for those
+    parameters) and, for AdamW's, ``exp_avg_sq``.
+
+    The update of a matrix needs all of it, so the optimizer runs after the last gradient bucket on every rank: it is
+    neither sharded nor run per bucket (a reducer that is given it for that raises)."""
+
+    _state_keys = ("momentum_buffer",)
+    graph_safe = True      # AdamW's step number lives on the device; lr changes force a re-capture
+
+    def __init__(self, model, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.1, ns_steps=5, ns_coeffs=K.NS_COEFFS,
+                 eps=1e-7, adjust_lr="match_rms_adamw", betas=(0.9, 0.95), adamw_eps=1e-8, use_muon=None):
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError("FusedMuon: momentum must be in [0, 1), got %r" % (momentum,))
+        if adjust_lr not in K.MUON_ADJUST:
+            raise ValueError("FusedMuon: adjust_lr must be one of %s, got %r" % (sorted(K.MUON_ADJUST), adjust_lr))
+        if len(betas) != 2 or not all(0.0 < b < 1.0 for b in betas):
+            raise ValueError("FusedMuon: betas must be two numbers in (0, 1), got %r" % (betas,))
+        if not adamw_eps > 0.0:
+            raise ValueError("FusedMuon: adamw_eps must be positive, got %r" % (adamw_eps,))
+        K._ns_check_schedule(ns_steps, ns_coeffs, eps)
+        arena = _arena_from(model)
+        last = max([i for i, p in enumerate(arena.params) if p.dim() >= 2], default=-1)
+        if use_muon is None:
+            self._muon = [i for i, p in enumerate(arena.params) if p.dim() >= 2 and i != last]
+        else:
+            self._muon = [i for i, p in enumerate(arena.params) if p.dim() >= 2 and use_muon(arena.names[i], p)]
+        is_muon = set(self._muon)
+        # AdamW's parameters: whole slots of the arena (padding included: it is zero and stays zero), their second
+        # moments packed in a buffer of their own
+        self._aux, at = [], 0
+        for i, p in enumerate(arena.params):
+            if i not in is_muon:
+                n = (p.numel() + 63) // 64 * 64
+                self._aux.append((i, arena.offsets[i], n, at))
+                at += n
+        self._exp_avg_sq = torch.zeros(max(at, 4), dtype=torch.float32, device=arena.device)
+        self._step_device = torch.zeros(1, dtype=torch.int32, device=arena.device)
+        super().__init__(model, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
+                                     ns_steps=ns_steps, ns_coeffs=tuple(ns_coeffs), eps=eps, adjust_lr=adjust_lr,
+                                     betas=tuple(betas), adamw_eps=adamw_eps))
+        self._table = (K.adamw_range_table([(o, n, v) for _, o, n, v in self._aux], arena.device)
+                       if self._aux and arena.device.type == "cuda" else None)
+
+    @property
+    def _sharded_by(self):
+        return None
+
+    @_sharded_by.setter
+    def _sharded_by(self, reducer):
+        if reducer is not None:
+            raise ValueError("FusedMuon updates whole matrices after the last gradient bucket: it can be neither sharded "
+                             "nor run per bucket (shard_optimizer / bucket_optimizer)")
+
+    def _exp_avg_sq_view(self, i, at):
+        p = self.arena.params[i]
+        v = self._exp_avg_sq[at:at + p.numel()].view(self.arena._mem_shape(i))
+        return v.permute(0, 3, 1, 2) if p.dim() == 4 else v
+
+    def _bind_state_views(self):
+        super()._bind_state_views()
+        for i, _, _, at in self._aux:
+            self.state[self.arena.params[i]]["exp_avg_sq"] = self._exp_avg_sq_view(i, at)
+
+    def load_state_dict(self, state_dict):
+        mine = {i for i, _, _, _ in self._aux}
+        for i, st in state_dict.get("state", {}).items():
+            if st and ("exp_avg_sq" in st) != (int(i) in mine):
+                raise ValueError("FusedMuon: the checkpoint divides the parameters between Muon and AdamW differently "
+                                 "(parameter %s)" % i)
+        super().load_state_dict(state_dict)
+        with torch.no_grad():
+            for i, _, _, at in self._aux:
+                st = self.state[self.arena.params[i]]
+                view = self._exp_avg_sq_view(i, at)
+                if torch.is_tensor(st.get("exp_avg_sq")) and st["exp_avg_sq"].data_ptr() != view.data_ptr():
+                    view.copy_(st["exp_avg_sq"])
+                st["exp_avg_sq"] = view
+            self._step_device.fill_(self._steps)
+
+    @torch.no_grad()
+    def step(self, closure=None, grad_scale=1.0):
+        loss = closure() if closure is not None else None
+        a, g = self.arena, self.param_groups[0]
+        self._check_arena()
+        mom = self._flat_state["momentum_buffer"]
+        mats = [a.params[i] for i in self._muon]
+        if a.flat_master.is_cuda:
+            a.collect_autograd_grads()
+            self._step_device.add_(1)
+            K.muon_step([a.mem2d(a.flat_master, p) for p in mats], [a.grad(p) for p in mats],
+                        [a.mem2d(mom, p) for p in mats], [a.lp(p) for p in mats], g["lr"], g["momentum"], g["nesterov"],
+                        g["weight_decay"], g["ns_steps"], g["ns_coeffs"], g["eps"], g["adjust_lr"], grad_scale)
+            if self._table is not None:
+                K.adamw_ranges(a.flat_master, a.flat_grad, mom, self._exp_avg_sq, a.flat_lp, self._table,
+                               self._step_device, g["lr"], g["betas"][0], g["betas"][1], g["adamw_eps"], g["weight_decay"],
+                               grad_scale)
+            a.lp_written_by_optimizer()
+        else:
+            a.gather_autograd_grads()
+            self._step_device.add_(1)
+            self._step_cpu(mats, mom, g, grad_scale)
+        self._steps += 1
+        return loss
+
+    def _step_cpu(self, mats, mom, g, grad_scale):
+        a, mu = self.arena, g["momentum"]
+        for p in mats:
+            w, m, d = a.mem2d(a.flat_master, p), a.mem2d(mom, p), a.grad(p).float() * grad_scale
+            m.mul_(mu).add_(d, alpha=1 - mu)
+            u = d.mul(1 - mu).add_(m, alpha=mu) if g["nesterov"] else m
+            o = _newton_schulz_cpu(u, g["ns_steps"], g["ns_coeffs"], g["eps"])
+            w.mul_(1 - g["lr"] * g["weight_decay"]).add_(o, alpha=-g["lr"] * K.MUON_ADJUST[g["adjust_lr"]](*w.shape))
+        (b1, b2), t = g["betas"], self._steps + 1
+        for i, o, n, at in self._aux:
+            w, m, v = a.flat_master[o:o + n], mom[o:o + n], self._exp_avg_sq[at:at + n]
+            d = a.flat_grad[o:o + n].float() * grad_scale
+            w.mul_(1 - g["lr"] * g["weight_decay"])
+            m.mul_(b1).add_(d, alpha=1 - b1)
+            v.mul_(b2).addcmul_(d, d, value=1 - b2)
+            denom = (v.sqrt() / math.sqrt(1 - b2 ** t)).add_(g["adamw_eps"])
+            w.addcdiv_(m, denom, value=-g["lr"] / (1 - b1 ** t))

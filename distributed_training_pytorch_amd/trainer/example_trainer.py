@@ -20,7 +20,7 @@ from ..data.image_folder import ExampleDataset
 from ..data.synthetic import SyntheticImageDataset
 from ..models.vgg16 import VGG16
 from ..ops.layers import SoftmaxCrossEntropy, top1_hits
-from ..ops.optim import FusedSGD
+from ..ops.optim import FusedMuon, FusedSGD
 from ..utils.profiler import trace_range
 from .trainer import Trainer
 
@@ -53,6 +53,8 @@ class ExampleTrainer(Trainer):
                  weight_decay=1e-4,
                  milestones=(50, 100, 200),
                  batch_norm=False,
+                 group_norm=0,
+                 optimizer="sgd",
                  grad_dtype=torch.float32,
                  fp8_classifier=False,
                  uint8_input=False,
@@ -66,6 +68,10 @@ class ExampleTrainer(Trainer):
         self.lr, self.momentum, self.weight_decay = lr, momentum, weight_decay
         self.milestones = list(milestones)
         self.batch_norm = batch_norm
+        self.group_norm = int(group_norm)            # groups of VGG16-GN's normalisation layers; 0: none
+        if optimizer not in ("sgd", "muon"):
+            raise ValueError("optimizer must be 'sgd' or 'muon', got %r" % (optimizer,))
+        self.optimizer_name = optimizer
         self.grad_dtype = grad_dtype
         self.fp8_classifier = fp8_classifier
         # ship uint8 pixels host->device and normalise inside the conv1 ingest kernel
@@ -102,7 +108,7 @@ class ExampleTrainer(Trainer):
 
     # model / loss / optimiser -----------------------------------------------------------------
     def build_model(self):
-        model = VGG16(3, len(self.labels), True, batch_norm=self.batch_norm, grad_dtype=self.grad_dtype,
+        model = VGG16(3, len(self.labels), True, batch_norm=self.batch_norm, group_norm=self.group_norm, grad_dtype=self.grad_dtype,
                       fp8_classifier=self.fp8_classifier)
         if self.uint8_input:
             model.set_input_normalization(*self.input_normalization())
@@ -121,6 +127,8 @@ class ExampleTrainer(Trainer):
         return SoftmaxCrossEntropy()
 
     def build_optimizer(self):
+        if self.optimizer_name == "muon":
+            return FusedMuon(self.model, lr=self.lr, weight_decay=self.weight_decay)
         return FusedSGD(self.model, lr=self.lr, momentum=self.momentum, weight_decay=self.weight_decay)
 
     def build_scheduler(self):

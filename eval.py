@@ -75,6 +75,7 @@ def main(argv=None):
     ap.add_argument("--batch-size", type=int, default=64)
     ap.add_argument("--device", default=DEVICE)
     ap.add_argument("--batch-norm", action="store_true")
+    ap.add_argument("--group-norm", type=int, default=0, metavar="GROUPS", help="the model was trained with main.py --group-norm")
     ap.add_argument("--fp8-classifier", action="store_true")
     ap.add_argument("--num-workers", type=int, default=0, help="DataLoader decode workers")
     ap.add_argument("--uint8-input", action="store_true",
@@ -84,7 +85,8 @@ def main(argv=None):
     labels = args.labels.split(",")
     device = torch.device(args.device)
 
-    model = VGG16(3, len(labels), True, batch_norm=args.batch_norm, fp8_classifier=args.fp8_classifier)
+    model = VGG16(3, len(labels), True, batch_norm=args.batch_norm, group_norm=args.group_norm,
+                  fp8_classifier=args.fp8_classifier)
     ckpt = load_snapshot(args.model)
     model.load_state_dict(ckpt["model_state_dict"])
     model = model.to(device)
