@@ -1182,13 +1182,46 @@ int fill_table(NsCall& c, int count, const int* rows, const int* cols) {
   return 0;
 }
 
+// A matrix whose products fill the chip by themselves (m above 1024) is worked off alone, the others of a call together:
+// 13.7 ms for all of VGG16's matrices, 18.9 with all 15 in every launch (XCDs whose tiles have a shorter K wait).
+// The parts follow one another on the stream and share the workspace.
+constexpr int NS_ALONE = 1024;
+
+template <class F> int each_part(const NsCall& all, F run) {
+  NsCall part = all;
+  int rc = 0, k = 0;
+  for (int i = 0; i < all.count; ++i) {
+    const NsMat& t = all.tb.mat[i];
+    if ((t.rows < t.cols ? t.rows : t.cols) > NS_ALONE) {
+      NsCall one = all;
+      one.count = 1;
+      one.tb.mat[0] = t;
+      if ((rc = run(one))) return rc;
+    } else {
+      part.tb.mat[k++] = t;
+    }
+  }
+  part.count = k;
+  return k ? run(part) : 0;
+}
+
+long ns_bytes(const NsCall& all) {
+  long most = 0;
+  each_part(all, [&](NsCall& c) {
+    const long n = ns_layout(c);
+    if (n > most) most = n;
+    return 0;
+  });
+  return most;
+}
+
 }  // namespace
 
 // Bytes of scratch for these matrices (at most 24 a call); 0: refused.
 extern "C" size_t dtp_ns_workspace(int count, const int* rows, const int* cols) {
   NsCall c;
   if (fill_table(c, count, rows, cols)) return 0;
-  return (size_t)ns_layout(c);
+  return (size_t)ns_bytes(c);
 }
 
 // out[i] = Newton-Schulz of src[i] ([rows][cols], contiguous).  in_kind / out_kind: 0 f32, 1 bf16, 2 f16.
@@ -1196,22 +1229,26 @@ extern "C" size_t dtp_ns_workspace(int count, const int* rows, const int* cols) 
 extern "C" int dtp_newton_schulz(int count, const void** src, void** out, const int* rows, const int* cols, int in_kind,
                                  int out_kind, int steps, const float* coeffs, const float* scales, float eps, void* ws,
                                  size_t ws_bytes, hipStream_t st) {
-  NsCall c;
-  int rc = fill_table(c, count, rows, cols);
+  NsCall all;
+  const int rc = fill_table(all, count, rows, cols);
   if (rc) return rc;
   if (steps < 1 || in_kind < 0 || in_kind > 2 || out_kind < 0 || out_kind > 2) return -12;
-  if ((size_t)ns_layout(c) > ws_bytes) return -13;
+  if ((size_t)ns_bytes(all) > ws_bytes) return -13;
   for (int i = 0; i < count; ++i) {
-    c.tb.mat[i].src = src[i];
-    c.tb.mat[i].out = out[i];
-    c.tb.mat[i].aligned = (((size_t)src[i] | (size_t)out[i]) & 15) == 0;
+    NsMat& t = all.tb.mat[i];
+    t.src = src[i];
+    t.out = out[i];
+    t.aligned = (((size_t)src[i] | (size_t)out[i]) & 15) == 0;
   }
   const MuonArgs ma = {};
-  c.ws = (char*)ws;
-  c.st = st;
-  return in_kind == 0 ? ns_run<0, 0>(c, ma, steps, coeffs, scales, eps, out_kind)
-         : in_kind == 1 ? ns_run<1, 0>(c, ma, steps, coeffs, scales, eps, out_kind)
-                        : ns_run<2, 0>(c, ma, steps, coeffs, scales, eps, out_kind);
+  all.ws = (char*)ws;
+  all.st = st;
+  return each_part(all, [&](NsCall& c) {
+    ns_layout(c);
+    return in_kind == 0 ? ns_run<0, 0>(c, ma, steps, coeffs, scales, eps, out_kind)
+           : in_kind == 1 ? ns_run<1, 0>(c, ma, steps, coeffs, scales, eps, out_kind)
+                          : ns_run<2, 0>(c, ma, steps, coeffs, scales, eps, out_kind);
+  });
 }
 
 // One Muon step: mom <- momentum*mom + (1-momentum)*grad; O = Newton-Schulz of (nesterov ? (1-momentum)*grad +
@@ -1220,19 +1257,22 @@ extern "C" int dtp_muon_step(int count, void** w, const void** grad, void** mom,
                              const int* cols, int grad_bf16, float momentum, int nesterov, float grad_scale,
                              const float* decay, const float* step, int steps, const float* coeffs, const float* scales,
                              float eps, void* ws, size_t ws_bytes, hipStream_t st) {
-  NsCall c;
-  int rc = fill_table(c, count, rows, cols);
+  NsCall all;
+  const int rc = fill_table(all, count, rows, cols);
   if (rc) return rc;
   if (steps < 1) return -12;
-  if ((size_t)ns_layout(c) > ws_bytes) return -13;
+  if ((size_t)ns_bytes(all) > ws_bytes) return -13;
   for (int i = 0; i < count; ++i) {
-    NsMat& t = c.tb.mat[i];
+    NsMat& t = all.tb.mat[i];
     t.src = grad[i]; t.mom = (float*)mom[i]; t.w = (float*)w[i]; t.out = lp[i];
     t.decay = decay[i]; t.step = step[i];
     t.aligned = (((size_t)grad[i] | (size_t)mom[i] | (size_t)w[i] | (size_t)lp[i]) & 15) == 0;
   }
   const MuonArgs ma = {momentum, 1.f - momentum, grad_scale, nesterov};
-  c.ws = (char*)ws;
-  c.st = st;
-  return grad_bf16 ? ns_run<1, 1>(c, ma, steps, coeffs, scales, eps, 3) : ns_run<0, 1>(c, ma, steps, coeffs, scales, eps, 3);
+  all.ws = (char*)ws;
+  all.st = st;
+  return each_part(all, [&](NsCall& c) {
+    ns_layout(c);
+    return grad_bf16 ? ns_run<1, 1>(c, ma, steps, coeffs, scales, eps, 3) : ns_run<0, 1>(c, ma, steps, coeffs, scales, eps, 3);
+  });
 }
