@@ -13,6 +13,8 @@
 // cancel (E[x^2] - mean^2 in f32 loses mean^2 / var * 6e-8).
 #include "dtp_common.h"
 
+#include <utility>
+
 namespace {
 
 constexpr int GN_MAXC = 4096;        // channels: a block's per-channel sums live in LDS (2 * C floats)
@@ -158,6 +160,13 @@ template <int VEC> DTP_DEVINL void groups_of(int c, int cpg, int* g) {
   }
 }
 
+// f(0), f(1), .. f(N - 1) with the number known where the body is compiled: as a loop, the kept words of some types came to
+// lie in one wide vector, copied at every row's condition (up to 3.5 KB a lane in scratch memory).
+template <class F, int... I> DTP_DEVINL void each_of(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F> DTP_DEVINL void each(F&& f) { each_of(f, std::make_integer_sequence<int, N>{}); }
+
 template <class T, int VEC, int NT, int KV>
 __global__ __launch_bounds__(NT) void gn_slab_fwd_kernel(const void* __restrict__ x_, const float* __restrict__ gamma,
                                                          const float* __restrict__ beta, void* __restrict__ y_,
@@ -174,11 +183,10 @@ __global__ __launch_bounds__(NT) void gn_slab_fwd_kernel(const void* __restrict_
   const size_t base = (size_t)n * s.HW * s.CV;
   const word* xn = (const word*)x_ + base + c0 / VEC;
   word w[KV];
-#pragma unroll
-  for (int i = 0; i < KV; ++i) {
+  each<KV>([&](auto i) {
     const int r = ty + i * R;
     if (ty < R && r < s.HW) w[i] = xn[(size_t)r * s.CV];
-  }
+  });
   float p[VEC], a0[VEC], a1[VEC];
   int gl[VEC];                                      // group within the slab
   groups_of<VEC>(tx * VEC, s.cpg, gl);
@@ -187,8 +195,7 @@ __global__ __launch_bounds__(NT) void gn_slab_fwd_kernel(const void* __restrict_
     p[e] = pivot_of<T, VEC>((const word*)x_ + base, g0 + gl[e], s.cpg);
     a0[e] = a1[e] = 0.f;
   }
-#pragma unroll
-  for (int i = 0; i < KV; ++i) {
+  each<KV>([&](auto i) {
     const int r = ty + i * R;
     if (ty < R && r < s.HW) {
       float f[VEC];
@@ -200,7 +207,7 @@ __global__ __launch_bounds__(NT) void gn_slab_fwd_kernel(const void* __restrict_
         a1[e] = fmaf(d, d, a1[e]);
       }
     }
-  }
+  });
   // neighbouring channels of one group and thread are one unit of u = gcd(cpg, VEC)
   int u = 1;
   if (VEC > 1 && s.cpg % 2 == 0) {
@@ -266,8 +273,7 @@ __global__ __launch_bounds__(NT) void gn_slab_fwd_kernel(const void* __restrict_
     be[e] = beta[c0 + e];
   }
   word* yn = (word*)y_ + base + c0 / VEC;
-#pragma unroll
-  for (int i = 0; i < KV; ++i) {
+  each<KV>([&](auto i) {
     const int r = ty + i * R;
     if (ty < R && r < s.HW) {
       float f[VEC], o[VEC];
@@ -276,7 +282,7 @@ __global__ __launch_bounds__(NT) void gn_slab_fwd_kernel(const void* __restrict_
       for (int e = 0; e < VEC; ++e) o[e] = act_fwd<T>(fmaf((f[e] - mu[e]) * rs[e], ga[e], be[e]), act);
       yn[(size_t)r * s.CV] = Pack<T, VEC>::pack(o);
     }
-  }
+  });
 }
 
 // sums: per-channel (sum dz, sum dz*xhat) of every image, [N][2][C], for gn_dparam_kernel
@@ -297,14 +303,13 @@ __global__ __launch_bounds__(NT) void gn_slab_bwd_kernel(const void* __restrict_
   const size_t base = (size_t)n * s.HW * s.CV + c0 / VEC;
   const word *xn = (const word*)x_ + base, *dn = (const word*)dy_ + base;
   word wx[KV], wd[KV];
-#pragma unroll
-  for (int i = 0; i < KV; ++i) {
+  each<KV>([&](auto i) {
     const int r = ty + i * R;
     if (ty < R && r < s.HW) {
       wx[i] = xn[(size_t)r * s.CV];
       wd[i] = dn[(size_t)r * s.CV];
     }
-  }
+  });
   float mu[VEC], rs[VEC], ga[VEC], be[VEC], a0[VEC], a1[VEC];
   int gl[VEC];
   groups_of<VEC>(tx * VEC, s.cpg, gl);
@@ -317,8 +322,7 @@ __global__ __launch_bounds__(NT) void gn_slab_bwd_kernel(const void* __restrict_
     be[e] = beta[c0 + e];
     a0[e] = a1[e] = 0.f;
   }
-#pragma unroll
-  for (int i = 0; i < KV; ++i) {
+  each<KV>([&](auto i) {
     const int r = ty + i * R;
     if (ty < R && r < s.HW) {
       float f[VEC], d[VEC];
@@ -332,7 +336,7 @@ __global__ __launch_bounds__(NT) void gn_slab_bwd_kernel(const void* __restrict_
         a1[e] = fmaf(dz, xh, a1[e]);
       }
     }
-  }
+  });
   int rows;
   const int mine = column_rows(TX, NT, ty, R, rows);
 #pragma unroll
@@ -376,8 +380,7 @@ __global__ __launch_bounds__(NT) void gn_slab_bwd_kernel(const void* __restrict_
     m2[e] = ms[2 * gl[e] + 1];
   }
   word* on = (word*)dx_ + base;
-#pragma unroll
-  for (int i = 0; i < KV; ++i) {
+  each<KV>([&](auto i) {
     const int r = ty + i * R;
     if (ty < R && r < s.HW) {
       float f[VEC], d[VEC], o[VEC];
@@ -391,7 +394,7 @@ __global__ __launch_bounds__(NT) void gn_slab_bwd_kernel(const void* __restrict_
       }
       on[(size_t)r * s.CV] = Pack<T, VEC>::pack(o);
     }
-  }
+  });
 }
 
 // ---------------------------------------------------------------------------------------------------------
