@@ -109,6 +109,7 @@ struct GnShape {
   int N, HW, C, G, cpg;      // cpg = C / G
   int CV;                    // C / VEC
   int chunks, rows;          // an image's rows in `chunks` pieces of `rows`
+  int once;                  // so many pieces from the front are read past the caches (GN_KEEP)
 };
 
 // The value around which a group's sums are taken: its first one in the image.
@@ -403,6 +404,20 @@ __global__ __launch_bounds__(NT) void gn_slab_bwd_kernel(const void* __restrict_
 // parameters stay in registers.
 constexpr int GN_T = 256;
 
+// Both passes over data that does not stay in the caches as a whole: the first reads from the front and the second from the
+// back; what lies before the last GN_KEEP bytes is read past the caches, so that those bytes are still in the 256 MB
+// last-level cache when the second pass comes to them; its results are written past the caches too.  Measured (us; in
+// order with plain loads and stores / from the back, results past the caches / and GN_KEEP 128, 224, 256, 320 MB): forward
+// 64x224x224x64 (411 MB) 272 / 253 / 216, 203, 204, 236, 256x224x224x64 - / 950 / 885, 859, 853, 916; backward
+// 64x112x112x128 (411 MB) 232 / 186 / 181, 175, 174, 184, 64x56x56x256 (206 MB, all kept) 104 / 92.  Both passes over as
+// many images at a time as the cache holds cost more in launches than it gains: 1120 for the 950.
+constexpr double GN_KEEP = 240.0 * (1 << 20);
+
+template <bool ONCE, class W> DTP_DEVINL W load_word(const W* p) {
+  if constexpr (ONCE) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+
 // BWD 0: per group (sum (x-p), sum (x-p)^2) -> partial [N][chunks][G][2]
 // BWD 1: per channel (sum dz, sum dz*xhat)  -> partial [N][chunks][2][C]
 template <class T, int VEC, int BWD>
@@ -440,29 +455,34 @@ __global__ __launch_bounds__(GN_T) void gn_partial_kernel(const void* __restrict
           p[e] = pivot_of<T, VEC>(xn, g, s.cpg);
         }
       }
+      const auto rows = [&](auto once) {
+        constexpr bool ONCE = decltype(once)::value;
 #pragma unroll 4
-      for (int r = r0 + ty; r < r1; r += R) {
-        float f[VEC];
-        Pack<T, VEC>::unpack(xn[(size_t)r * s.CV + cv], f);
-        if (BWD) {
-          float d[VEC];
-          Pack<T, VEC>::unpack(dn[(size_t)r * s.CV + cv], d);
+        for (int r = r0 + ty; r < r1; r += R) {
+          float f[VEC];
+          Pack<T, VEC>::unpack(load_word<ONCE>(xn + (size_t)r * s.CV + cv), f);
+          if (BWD) {
+            float d[VEC];
+            Pack<T, VEC>::unpack(load_word<ONCE>(dn + (size_t)r * s.CV + cv), d);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float xh = (f[e] - p[e]) * rs[e];
-            const float dz = act_bwd<T>(fmaf(xh, ga[e], be[e]), d[e], act);
-            a0[e] += dz;
-            a1[e] = fmaf(dz, xh, a1[e]);
-          }
-        } else {
+            for (int e = 0; e < VEC; ++e) {
+              const float xh = (f[e] - p[e]) * rs[e];
+              const float dz = act_bwd<T>(fmaf(xh, ga[e], be[e]), d[e], act);
+              a0[e] += dz;
+              a1[e] = fmaf(dz, xh, a1[e]);
+            }
+          } else {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float d = f[e] - p[e];
-            a0[e] += d;
-            a1[e] = fmaf(d, d, a1[e]);
+            for (int e = 0; e < VEC; ++e) {
+              const float d = f[e] - p[e];
+              a0[e] += d;
+              a1[e] = fmaf(d, d, a1[e]);
+            }
           }
         }
-      }
+      };
+      if ((int)blockIdx.x < s.once) rows(std::true_type{});
+      else rows(std::false_type{});
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         thr[(ty * TX + tx) * VEC + e] = a0[e];
@@ -616,7 +636,8 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(const void* __restrict__
                                                         const float* __restrict__ stats, const float* __restrict__ coef,
                                                         void* __restrict__ out_, const GnShape s, const int act) {
   typedef typename Pack<T, VEC>::word word;
-  const int n = blockIdx.x / s.chunks, chunk = blockIdx.x - n * s.chunks;
+  const int block = gridDim.x - 1 - blockIdx.x;      // the pieces read last first
+  const int n = block / s.chunks, chunk = block - n * s.chunks;
   const int r0 = chunk * s.rows, r1 = min(s.HW, r0 + s.rows);
   const size_t base = (size_t)n * s.HW * s.CV;
   const word* xn = (const word*)x_ + base;
@@ -637,31 +658,36 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(const void* __restrict__
       be[e] = beta[c];
       if (BWD) { m1[e] = coef[gi]; m2[e] = coef[gi + 1]; }
     }
+    const auto rows = [&](auto once) {
+      constexpr bool ONCE = decltype(once)::value;
 #pragma unroll 4
-    for (int r = r0 + ty; r < r1; r += R) {
-      float f[VEC], o[VEC];
-      Pack<T, VEC>::unpack(xn[(size_t)r * s.CV + cv], f);
-      if (BWD) {
-        float d[VEC];
-        Pack<T, VEC>::unpack(dn[(size_t)r * s.CV + cv], d);
+    for   (int r = r0 + ty; r < r1; r += R) {
+        float f[VEC], o[VEC];
+        Pack<T, VEC>::unpack(load_word<ONCE>(xn + (size_t)r * s.CV + cv), f);
+        if (BWD) {
+          float d[VEC];
+          Pack<T, VEC>::unpack(load_word<ONCE>(dn + (size_t)r * s.CV + cv), d);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float xh = (f[e] - mu[e]) * rs[e];
-          const float dz = act_bwd<T>(fmaf(xh, ga[e], be[e]), d[e], act);
-          o[e] = rs[e] * (fmaf(ga[e], dz, -m1[e]) - xh * m2[e]);
+          for (int e = 0; e < VEC; ++e) {
+            const float xh = (f[e] - mu[e]) * rs[e];
+            const float dz = act_bwd<T>(fmaf(xh, ga[e], be[e]), d[e], act);
+            o[e] = rs[e] * (fmaf(ga[e], dz, -m1[e]) - xh * m2[e]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) o[e] = act_fwd<T>(fmaf((f[e] - mu[e]) * rs[e], ga[e], be[e]), act);
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) o[e] = act_fwd<T>(fmaf((f[e] - mu[e]) * rs[e], ga[e], be[e]), act);
+        __builtin_nontemporal_store(Pack<T, VEC>::pack(o), &on[(size_t)r * s.CV + cv]);
       }
-      on[(size_t)r * s.CV + cv] = Pack<T, VEC>::pack(o);
-    }
+    };
+    if (block < s.once) rows(std::true_type{});
+    else rows(std::false_type{});
   }
 }
 
 // Pieces of an image: about 2,048 blocks in all (8 a CU), but no piece under 32 KB, where a block's fixed part
 // (parameters, LDS fold) would outweigh its rows.
-GnShape shape_of(int N, int HW, int C, int G, int vec, int elem) {
+GnShape shape_of(int N, int HW, int C, int G, int vec, int elem, int bwd) {
   GnShape s;
   s.N = N; s.HW = HW; s.C = C; s.G = G; s.cpg = C / G; s.CV = C / vec;
   long want = (2048 + N - 1) / N;
@@ -671,6 +697,8 @@ GnShape shape_of(int N, int HW, int C, int G, int vec, int elem) {
   if (want < 1) want = 1;
   s.rows = (int)((HW + want - 1) / want);
   s.chunks = (HW + s.rows - 1) / s.rows;
+  const double all = (double)N * HW * C * elem * (1 + bwd);
+  s.once = all <= GN_KEEP ? 0 : (int)((double)N * s.chunks * (1.0 - GN_KEEP / all));
   return s;
 }
 
@@ -730,6 +758,15 @@ int slab_groups(const GnShape& s, int vec, int elem, int bwd, int& threads) {
   return best;
 }
 
+// A launch holds fewer than 2^32 threads.
+bool grids_fit(const GnShape& s, int vec, int elem, int bwd) {
+  int nt;
+  const int sg = slab_groups(s, vec, elem, bwd, nt);
+  long most = sg ? (long)s.N * ((s.G + sg - 1) / sg) * nt : (long)s.N * s.chunks * GN_T;
+  if (!sg) most = max(most, bwd ? (long)s.N * GN_FOLD : ((long)s.N * s.G + 3) / 4 * 256);
+  return most < 1L << 32;
+}
+
 size_t partial_floats(const GnShape& s, int bwd) {
   return bwd ? (size_t)s.N * s.chunks * 2 * s.C : (size_t)s.N * s.chunks * s.G * 2;
 }
@@ -743,7 +780,7 @@ int gn_run_fwd(const void* x, const float* gamma, const float* beta, void* y, fl
   if (sl.SG) {
     sl.slabs = (s.G + sl.SG - 1) / sl.SG;
     const size_t lds = slab_lds(s, VEC, sl.SG, NT, 0);
-    const dim3 g((unsigned)(s.N * sl.slabs));
+    const dim3 g((unsigned)((long)s.N * sl.slabs));
     if (NT == 256) hipLaunchKernelGGL((gn_slab_fwd_kernel<T, VEC, 256, 8>), g, dim3(256), lds, st, x, gamma, beta, y, stats, s, sl, eps, act);
     else if (NT == 512) hipLaunchKernelGGL((gn_slab_fwd_kernel<T, VEC, 512, 16>), g, dim3(512), lds, st, x, gamma, beta, y, stats, s, sl, eps, act);
     else hipLaunchKernelGGL((gn_slab_fwd_kernel<T, VEC, 1024, 16>), g, dim3(1024), lds, st, x, gamma, beta, y, stats, s, sl, eps, act);
@@ -771,7 +808,7 @@ int gn_run_bwd(const void* x, const void* dy, const float* gamma, const float* b
   if (sl.SG) {
     sl.slabs = (s.G + sl.SG - 1) / sl.SG;
     const size_t slds = slab_lds(s, VEC, sl.SG, NT, 1);
-    const dim3 g((unsigned)(s.N * sl.slabs));
+    const dim3 g((unsigned)((long)s.N * sl.slabs));
     if (NT == 256) hipLaunchKernelGGL((gn_slab_bwd_kernel<T, VEC, 256, 8>), g, dim3(256), slds, st, x, dy, gamma, beta, stats, dx, sums, s, sl, act);
     else hipLaunchKernelGGL((gn_slab_bwd_kernel<T, VEC, 512, 16>), g, dim3(512), slds, st, x, dy, gamma, beta, stats, dx, sums, s, sl, act);
     hipLaunchKernelGGL(gn_dparam_kernel, dim3((s.C + 15) / 16), dim3(256), 0, st, sums, s.N, s.C, dgamma, dbeta, out_fp32,
@@ -814,7 +851,8 @@ int gn_run_bwd(const void* x, const void* dy, const float* gamma, const float* b
 extern "C" size_t dtp_gn_workspace(int N, int HW, int C, int G, int dtype, int bwd) {
   if (!gn_ok(N, HW, C, G, dtype, 0)) return (size_t)-1;
   const int elem = dtype == 2 ? 4 : 2, vec = gn_vec(C, elem);
-  const GnShape s = shape_of(N, HW, C, G, vec, elem);
+  const GnShape s = shape_of(N, HW, C, G, vec, elem, bwd);
+  if (!grids_fit(s, vec, elem, bwd)) return (size_t)-1;
   int nt;
   const size_t sums = bwd ? (size_t)N * 2 * C : 0;
   if (slab_groups(s, vec, elem, bwd, nt)) return sums;
@@ -826,7 +864,8 @@ extern "C" int dtp_gn_fwd(const void* x, const float* gamma, const float* beta, 
                           size_t ws_floats, int N, int HW, int C, int G, int dtype, int act, float eps, hipStream_t st) {
   if (!gn_ok(N, HW, C, G, dtype, act)) return -10;
   const int elem = dtype == 2 ? 4 : 2, vec = gn_vec(C, elem);
-  const GnShape s = shape_of(N, HW, C, G, vec, elem);
+  const GnShape s = shape_of(N, HW, C, G, vec, elem, 0);
+  if (!grids_fit(s, vec, elem, 0)) return -10;
   GN_DISPATCH(gn_run_fwd, x, gamma, beta, y, stats, ws, ws_floats, s, eps, act, st);
 }
 
@@ -836,6 +875,7 @@ extern "C" int dtp_gn_bwd(const void* x, const void* dy, const float* gamma, con
                           size_t ws_floats, int N, int HW, int C, int G, int dtype, int act, hipStream_t st) {
   if (!gn_ok(N, HW, C, G, dtype, act)) return -10;
   const int elem = dtype == 2 ? 4 : 2, vec = gn_vec(C, elem);
-  const GnShape s = shape_of(N, HW, C, G, vec, elem);
+  const GnShape s = shape_of(N, HW, C, G, vec, elem, 1);
+  if (!grids_fit(s, vec, elem, 1)) return -10;
   GN_DISPATCH(gn_run_bwd, x, dy, gamma, beta, stats, dx, dgamma, dbeta, out_fp32, beta_g, beta_b, ws, ws_floats, s, act, st);
 }

@@ -997,7 +997,7 @@ def _gn_check(x, groups, act, *vecs):
 def _gn_workspace(N, HW, C, G, dt, bwd):
     n = _lib.hip().dtp_gn_workspace(N, HW, C, G, dt, bwd)
     if n == (1 << (8 * _ctypes.sizeof(_ctypes.c_size_t))) - 1:
-        raise RuntimeError("group norm: the native library refuses [%d, %d, %d] in %d groups" % (N, HW, C, G))
+        raise ValueError("group norm: the native library refuses [%d, %d, %d] in %d groups" % (N, HW, C, G))
     return n
 
 

@@ -30,3 +30,13 @@ def _fwd(x, groups=4, act="relu", gamma=None, beta=None):
 def test_gn_refusals(call, what):
     with pytest.raises(ValueError, match=what):
         call()
+
+
+@pytest.mark.parametrize("bwd", [0, 1])
+def test_more_threads_than_a_launch_holds(bwd):
+    """2^24 one-pixel images and up: 256 threads each are 2^32 (4 million are fine: their groups fit one slab)."""
+    assert K._gn_workspace(1 << 22, 1, 32, 4, 0, bwd) == bwd * (1 << 22) * 64
+    with pytest.raises(ValueError, match="refuses"):
+        K._gn_workspace(1 << 24, 1, 32, 4, 0, bwd)
+    with pytest.raises(ValueError, match="refuses"):
+        K._gn_workspace(1 << 22, 1, 4096, 4096, 0, bwd)

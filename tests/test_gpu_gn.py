@@ -120,6 +120,13 @@ def test_gn_fwd(shape, groups, dtype, act):
     _check(y, ref, 1.1 * zmag, "y")
 
 
+def test_gn_data_beyond_the_caches():
+    """272 MB (backward: 544 MB): more than the last-level cache, read past it up to the last 240 MiB.  The same bounds
+    as the small shapes: a thread adds 74 rows."""
+    test_gn_fwd((6, 381, 331, 180), 12, BF16, "relu")
+    test_gn_bwd((6, 381, 331, 180), 12, BF16, "silu")
+
+
 @pytest.mark.parametrize("act", ["none", "relu", "silu"])
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("shape,groups", SHAPES)
