@@ -85,18 +85,23 @@ template <class T> DTP_DEVINL float sigmoid(float z) {
   if constexpr (T::size == 4) return 1.f / (1.f + expf(-z));
   else return __builtin_amdgcn_rcpf(1.f + __expf(-z));
 }
-template <class T> DTP_DEVINL float act_fwd(float z, int act) {
-  if (act == ACT_RELU) return z <= 0.f ? 0.f : z;            // NaN stays NaN
-  if (act == ACT_SILU) return z * sigmoid<T>(z);
-  return z;
+template <class T, int ACT> DTP_DEVINL float act_fwd(float z) {
+  if constexpr (ACT == ACT_RELU) return z <= 0.f ? 0.f : z;            // NaN stays NaN
+  else if constexpr (ACT == ACT_SILU) return z * sigmoid<T>(z);
+  else return z;
 }
-template <class T> DTP_DEVINL float act_bwd(float z, float dy, int act) {
-  if (act == ACT_RELU) return z > 0.f ? dy : 0.f;
-  if (act == ACT_SILU) {
+template <class T, int ACT> DTP_DEVINL float act_bwd(float z, float dy) {
+  if constexpr (ACT == ACT_RELU) return z > 0.f ? dy : 0.f;
+  else if constexpr (ACT == ACT_SILU) {
     const float s = sigmoid<T>(z);
     return dy * s * (1.f + z * (1.f - s));
-  }
-  return dy;
+  } else return dy;
+}
+// f(activation), chosen once for all rows (a choice at every value: backward 64x28x28x512 53 us, now 43)
+template <class F> DTP_DEVINL void with_act(int act, F&& f) {
+  if (act == ACT_RELU) f(std::integral_constant<int, ACT_RELU>{});
+  else if (act == ACT_SILU) f(std::integral_constant<int, ACT_SILU>{});
+  else f(std::integral_constant<int, ACT_NONE>{});
 }
 
 DTP_DEVINL double wave_reduce_sum_f64(double v) {
@@ -274,15 +279,18 @@ __global__ __launch_bounds__(NT) void gn_slab_fwd_kernel(const void* __restrict_
     be[e] = beta[c0 + e];
   }
   word* yn = (word*)y_ + base + c0 / VEC;
-  each<KV>([&](auto i) {
-    const int r = ty + i * R;
-    if (ty < R && r < s.HW) {
-      float f[VEC], o[VEC];
-      Pack<T, VEC>::unpack(w[i], f);
+  with_act(act, [&](auto which) {
+    constexpr int ACT = decltype(which)::value;
+    each<KV>([&](auto i) {
+      const int r = ty + i * R;
+      if (ty < R && r < s.HW) {
+        float f[VEC], o[VEC];
+        Pack<T, VEC>::unpack(w[i], f);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o[e] = act_fwd<T>(fmaf((f[e] - mu[e]) * rs[e], ga[e], be[e]), act);
-      yn[(size_t)r * s.CV] = Pack<T, VEC>::pack(o);
-    }
+        for (int e = 0; e < VEC; ++e) o[e] = act_fwd<T, ACT>(fmaf((f[e] - mu[e]) * rs[e], ga[e], be[e]));
+        yn[(size_t)r * s.CV] = Pack<T, VEC>::pack(o);
+      }
+    });
   });
 }
 
@@ -323,20 +331,23 @@ __global__ __launch_bounds__(NT) void gn_slab_bwd_kernel(const void* __restrict_
     be[e] = beta[c0 + e];
     a0[e] = a1[e] = 0.f;
   }
-  each<KV>([&](auto i) {
-    const int r = ty + i * R;
-    if (ty < R && r < s.HW) {
-      float f[VEC], d[VEC];
-      Pack<T, VEC>::unpack(wx[i], f);
-      Pack<T, VEC>::unpack(wd[i], d);
+  with_act(act, [&](auto which) {
+    constexpr int ACT = decltype(which)::value;
+    each<KV>([&](auto i) {
+      const int r = ty + i * R;
+      if (ty < R && r < s.HW) {
+        float f[VEC], d[VEC];
+        Pack<T, VEC>::unpack(wx[i], f);
+        Pack<T, VEC>::unpack(wd[i], d);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float xh = (f[e] - mu[e]) * rs[e];
-        const float dz = act_bwd<T>(fmaf(xh, ga[e], be[e]), d[e], act);
-        a0[e] += dz;
-        a1[e] = fmaf(dz, xh, a1[e]);
+        for (int e = 0; e < VEC; ++e) {
+          const float xh = (f[e] - mu[e]) * rs[e];
+          const float dz = act_bwd<T, ACT>(fmaf(xh, ga[e], be[e]), d[e]);
+          a0[e] += dz;
+          a1[e] = fmaf(dz, xh, a1[e]);
+        }
       }
-    }
+    });
   });
   int rows;
   const int mine = column_rows(TX, NT, ty, R, rows);
@@ -381,20 +392,23 @@ __global__ __launch_bounds__(NT) void gn_slab_bwd_kernel(const void* __restrict_
     m2[e] = ms[2 * gl[e] + 1];
   }
   word* on = (word*)dx_ + base;
-  each<KV>([&](auto i) {
-    const int r = ty + i * R;
-    if (ty < R && r < s.HW) {
-      float f[VEC], d[VEC], o[VEC];
-      Pack<T, VEC>::unpack(wx[i], f);
-      Pack<T, VEC>::unpack(wd[i], d);
+  with_act(act, [&](auto which) {
+    constexpr int ACT = decltype(which)::value;
+    each<KV>([&](auto i) {
+      const int r = ty + i * R;
+      if (ty < R && r < s.HW) {
+        float f[VEC], d[VEC], o[VEC];
+        Pack<T, VEC>::unpack(wx[i], f);
+        Pack<T, VEC>::unpack(wd[i], d);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float xh = (f[e] - mu[e]) * rs[e];
-        const float dz = act_bwd<T>(fmaf(xh, ga[e], be[e]), d[e], act);
-        o[e] = rs[e] * (fmaf(ga[e], dz, -m1[e]) - xh * m2[e]);
+        for (int e = 0; e < VEC; ++e) {
+          const float xh = (f[e] - mu[e]) * rs[e];
+          const float dz = act_bwd<T, ACT>(fmaf(xh, ga[e], be[e]), d[e]);
+          o[e] = rs[e] * (fmaf(ga[e], dz, -m1[e]) - xh * m2[e]);
+        }
+        on[(size_t)r * s.CV] = Pack<T, VEC>::pack(o);
       }
-      on[(size_t)r * s.CV] = Pack<T, VEC>::pack(o);
-    }
+    });
   });
 }
 
@@ -455,8 +469,9 @@ __global__ __launch_bounds__(GN_T) void gn_partial_kernel(const void* __restrict
           p[e] = pivot_of<T, VEC>(xn, g, s.cpg);
         }
       }
-      const auto rows = [&](auto once) {
+      const auto rows = [&](auto once, auto which) {
         constexpr bool ONCE = decltype(once)::value;
+        constexpr int ACT = decltype(which)::value;
 #pragma unroll 4
         for (int r = r0 + ty; r < r1; r += R) {
           float f[VEC];
@@ -467,7 +482,7 @@ __global__ __launch_bounds__(GN_T) void gn_partial_kernel(const void* __restrict
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
               const float xh = (f[e] - p[e]) * rs[e];
-              const float dz = act_bwd<T>(fmaf(xh, ga[e], be[e]), d[e], act);
+              const float dz = act_bwd<T, ACT>(fmaf(xh, ga[e], be[e]), d[e]);
               a0[e] += dz;
               a1[e] = fmaf(dz, xh, a1[e]);
             }
@@ -481,8 +496,10 @@ __global__ __launch_bounds__(GN_T) void gn_partial_kernel(const void* __restrict
           }
         }
       };
-      if ((int)blockIdx.x < s.once) rows(std::true_type{});
-      else rows(std::false_type{});
+      with_act(BWD ? act : ACT_NONE, [&](auto which) {
+        if ((int)blockIdx.x < s.once) rows(std::true_type{}, which);
+        else rows(std::false_type{}, which);
+      });
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         thr[(ty * TX + tx) * VEC + e] = a0[e];
@@ -658,8 +675,9 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(const void* __restrict__
       be[e] = beta[c];
       if (BWD) { m1[e] = coef[gi]; m2[e] = coef[gi + 1]; }
     }
-    const auto rows = [&](auto once) {
+    const auto rows = [&](auto once, auto which) {
       constexpr bool ONCE = decltype(once)::value;
+      constexpr int ACT = decltype(which)::value;
 #pragma unroll 4
     for   (int r = r0 + ty; r < r1; r += R) {
         float f[VEC], o[VEC];
@@ -670,18 +688,20 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(const void* __restrict__
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
             const float xh = (f[e] - mu[e]) * rs[e];
-            const float dz = act_bwd<T>(fmaf(xh, ga[e], be[e]), d[e], act);
+            const float dz = act_bwd<T, ACT>(fmaf(xh, ga[e], be[e]), d[e]);
             o[e] = rs[e] * (fmaf(ga[e], dz, -m1[e]) - xh * m2[e]);
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) o[e] = act_fwd<T>(fmaf((f[e] - mu[e]) * rs[e], ga[e], be[e]), act);
+          for (int e = 0; e < VEC; ++e) o[e] = act_fwd<T, ACT>(fmaf((f[e] - mu[e]) * rs[e], ga[e], be[e]));
         }
         __builtin_nontemporal_store(Pack<T, VEC>::pack(o), &on[(size_t)r * s.CV + cv]);
       }
     };
-    if (block < s.once) rows(std::true_type{});
-    else rows(std::false_type{});
+    with_act(act, [&](auto which) {
+      if (block < s.once) rows(std::true_type{}, which);
+      else rows(std::false_type{}, which);
+    });
   }
 }
 
@@ -722,22 +742,30 @@ size_t slab_lds(const GnShape& s, int vec, int sg, int nt, int bwd) {
   return (row + (bwd ? (size_t)2 * sg * s.cpg : 0) + 2 * (size_t)sg) * sizeof(float);
 }
 
+// rows of a thread
+long slab_rows(const GnShape& s, int vec, int sg, int nt) {
+  const long tx = (long)sg * s.cpg / vec;
+  return (s.HW + nt / tx - 1) / (nt / tx);
+}
+
 // Whether a slab of `sg` groups fits (columns, rows a thread, 64 KB of LDS): 0 no, else the threads
 int slab_fits(const GnShape& s, int vec, int sg, int bwd) {
-  static const int nt[3] = {256, 512, 1024}, kv[2][3] = {{8, 16, 16}, {8, 16, 0}};
+  static const int nt[3] = {256, 512, 1024}, kv[2][3] = {{8, 16, 14}, {8, 16, 0}};
   const long tx = (long)sg * s.cpg / vec;
   for (int v = 0; v < 3; ++v)
-    if (kv[bwd][v] && tx <= nt[v] && (s.HW + nt[v] / tx - 1) / (nt[v] / tx) <= kv[bwd][v] &&
+    if (kv[bwd][v] && tx <= nt[v] && slab_rows(s, vec, sg, nt[v]) <= kv[bwd][v] &&
         slab_lds(s, vec, sg, nt[v], bwd) <= 65536)
       return nt[v];
   return 0;
 }
 
 // Groups of a slab; 0: none fits, or its rows are so short (64 bytes, 32, 16) that the loads cost more than a second
-// pass.  Rows should be whole cache lines, but the workgroups 512 at least.  Measured (us, slab / two passes; bf16, 32
-// groups): rows of 64 bytes and more always pay (forward 64x56x56x256 41 / 67, backward 64x28x28x512 55 / 88); of 32:
-// forward 4x28x28x512 9 / 19, backward the same 18.5 / 45, but backward 64x56x56x256 146 / 118; of 16: 4x56x56x256
-// forward 12 / 19, backward 23 / 44, but forward 64x112x112x128 182 / 127.
+// pass.  Rows should be whole cache lines, but every CU should have a workgroup (16x56x56x256 with 256 at least, rows of
+// 32 bytes: forward 16 us, backward 26; with 512, rows of 16: 21 and 41).  Measured (us, slab / two passes; bf16 where
+// nothing else stands, 32 groups): rows of 64 bytes and more always pay (forward 64x56x56x256 38 / 66, backward
+// 64x28x28x512 43 / 58); of 32: forward 32x56x56x256 in f32 36 / 58, backward 32x56x56x256 47 / 55, but backward
+// 64x56x56x256 118 / 90; of 16: forward 8x56x56x256 14 / 19, 16x112x112x128 37 / 43, but 64x112x112x128 179 / 109 and, on
+// half of the CUs, 4x112x112x128 22 / 19; backward 8x56x56x256 23 / 26, but 16x80x80x256 66 / 58.
 int slab_groups(const GnShape& s, int vec, int elem, int bwd, int& threads) {
   const int step = vec / gcd(s.cpg, vec);            // groups that make whole vectors
   const long total = (long)s.N * s.HW * s.C * elem;
@@ -746,15 +774,16 @@ int slab_groups(const GnShape& s, int vec, int elem, int bwd, int& threads) {
     const int f = slab_fits(s, vec, sg, bwd);
     if (!f) break;
     const long blocks = (long)s.N * ((s.G + sg - 1) / sg), bytes = (long)sg * s.cpg * elem;
-    if (best && (blocks < 512 || bytes > 128)) break;
+    if (best && (blocks < 256 || bytes > 128)) break;
     best = sg;
     threads = f;
     if (bytes >= 128) break;
   }
   if (!best || best == s.G) return best;
-  const long bytes = (long)best * s.cpg * elem;
-  if (bytes < 32) return total <= (8L << 20) ? best : 0;
-  if (bytes < 64 && bwd) return total <= (32L << 20) ? best : 0;
+  const long bytes = (long)best * s.cpg * elem, blocks = (long)s.N * ((s.G + best - 1) / best);
+  if (bytes < 32 && total > (8L << 20) && blocks < 256) return 0;
+  if (bytes < 32 && total > ((bwd ? 16L : 56L) << 20)) return 0;
+  if (bytes < 64 && bwd && total > (64L << 20)) return 0;
   return best;
 }
 
@@ -783,7 +812,7 @@ int gn_run_fwd(const void* x, const float* gamma, const float* beta, void* y, fl
     const dim3 g((unsigned)((long)s.N * sl.slabs));
     if (NT == 256) hipLaunchKernelGGL((gn_slab_fwd_kernel<T, VEC, 256, 8>), g, dim3(256), lds, st, x, gamma, beta, y, stats, s, sl, eps, act);
     else if (NT == 512) hipLaunchKernelGGL((gn_slab_fwd_kernel<T, VEC, 512, 16>), g, dim3(512), lds, st, x, gamma, beta, y, stats, s, sl, eps, act);
-    else hipLaunchKernelGGL((gn_slab_fwd_kernel<T, VEC, 1024, 16>), g, dim3(1024), lds, st, x, gamma, beta, y, stats, s, sl, eps, act);
+    else hipLaunchKernelGGL((gn_slab_fwd_kernel<T, VEC, 1024, 14>), g, dim3(1024), lds, st, x, gamma, beta, y, stats, s, sl, eps, act);
     return DTP_CHECK_LAUNCH();
   }
   if (ws_floats < partial_floats(s, 0)) return -12;
