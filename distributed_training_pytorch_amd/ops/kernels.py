@@ -1036,6 +1036,8 @@ def gn_bwd(x, dy, gamma, beta, stats, groups, dgamma, dbeta, act="relu", beta_g=
             or dbeta.numel() != C or not dgamma.is_contiguous() or not dbeta.is_contiguous() \
             or dgamma.device != x.device or dbeta.device != x.device:
         raise ValueError("gn_bwd: dgamma / dbeta must be contiguous [C] of one dtype (f32 / bf16) on x's device")
+    if dgamma.data_ptr() == dbeta.data_ptr():
+        raise ValueError("gn_bwd: dgamma and dbeta share their memory")
     dx = torch.empty_like(x)
     if N == 0:
         if beta_g == 0.0:
@@ -1149,9 +1151,11 @@ def adamw_ranges(p, g, m, v, lp, table, step, lr, beta1, beta2, eps, wd, grad_sc
         raise ValueError("adamw_ranges: step must be a device int32, table adamw_range_table's")
     if not (0.0 < beta1 < 1.0 and 0.0 < beta2 < 1.0):
         raise ValueError("adamw_ranges: betas must be in (0, 1), got %r, %r" % (beta1, beta2))
-    check(_lib.hip().dtp_adamw_ranges(ptr(p), ptr(g), int(g.dtype == BF16), ptr(m), ptr(v), ptr(lp), ptr(table),
-                                      table.shape[0], ptr(step), float(lr), float(beta1), float(beta2), _math.log(beta1),
-                                      _math.log(beta2), float(eps), float(wd), float(grad_scale), stream()), "adamw_ranges")
+    with _on_device_of(p):
+        check(_lib.hip().dtp_adamw_ranges(ptr(p), ptr(g), int(g.dtype == BF16), ptr(m), ptr(v), ptr(lp), ptr(table),
+                                          table.shape[0], ptr(step), float(lr), float(beta1), float(beta2), _math.log(beta1),
+                                          _math.log(beta2), float(eps), float(wd), float(grad_scale), stream()),
+              "adamw_ranges")
 
 
 # ------------------------------------------------------------------------------------- Muon
@@ -1296,7 +1300,7 @@ def muon_step(params, grads, bufs, lps, lr, momentum=0.95, nesterov=True, weight
         raise ValueError("muon_step: %d params, %d grads, %d bufs, %d lps" % (n, len(grads), len(bufs), len(lps)))
     if n == 0:
         return
-    written = set()
+    spans = []
     for p, g, m, lp in zip(params, grads, bufs, lps):
         if p.dim() != 2 or p.dtype != torch.float32 or m.dtype != torch.float32 or g.dtype != grads[0].dtype \
                 or g.dtype not in (torch.float32, BF16) or (lp is not None and lp.dtype != BF16):
@@ -1304,13 +1308,19 @@ def muon_step(params, grads, bufs, lps, lr, momentum=0.95, nesterov=True, weight
         for t in (p, g, m) + ((lp,) if lp is not None else ()):
             if t.shape != p.shape or t.device != params[0].device or not t.is_contiguous():
                 raise ValueError("muon_step: params, grads, bufs and lps must agree in shape and device and be contiguous")
-        for t in (p, m) + ((lp,) if lp is not None else ()):
-            if t.numel() and t.data_ptr() in written:
-                raise ValueError("muon_step: a tensor that is written appears twice")
-            written.add(t.data_ptr())
-        if g.numel() and g.data_ptr() in (p.data_ptr(), m.data_ptr()):
-            raise ValueError("muon_step: a gradient shares its memory with what is written")
+        for t, out in ((g, False), (p, True), (m, True), (lp, True)):
+            if t is not None and t.numel():
+                at = t.data_ptr()
+                spans.append((at, at + t.numel() * t.element_size(), out))
         _ns_check_sides(p.shape[0], p.shape[1])
+    spans.sort()
+    end, written = 0, 0                       # of what begins before: the furthest end, and that of what is written
+    for lo, hi, out in spans:
+        if lo < (end if out else written):
+            raise ValueError("muon_step: a tensor that is written appears twice or shares its memory with another")
+        end = max(end, hi)
+        if out:
+            written = max(written, hi)
     if not params[0].is_cuda:
         raise ValueError("muon_step: CUDA tensors")
     jobs = [j for j in zip(params, grads, bufs, lps) if j[0].numel()]

@@ -261,3 +261,12 @@ def test_gn_empty_batch():
     dx = k.gn_bwd(x, x, ga, ga, st, 4, dg, db, beta_b=1.0)
     assert y.shape == x.shape == dx.shape and st.shape == (0, 4, 2)
     assert (dg == 0).all() and (db == 5).all()
+
+
+def test_gn_bwd_refuses_one_tensor_for_both_parameter_gradients():
+    k = _k()
+    x, dy, gamma, beta = _inputs((2, 3, 3, 16), BF16)
+    _, stats = k.gn_fwd(x, gamma, beta, 4)
+    d = torch.zeros(16, device="cuda")
+    with pytest.raises(ValueError, match="share their memory"):
+        k.gn_bwd(x, dy, gamma, beta, stats, 4, d, d)

@@ -46,6 +46,31 @@ def test_muon_refuses_what_is_written_twice():
         K.muon_step([p], [m], [m], [None], lr=0.1)
 
 
+@pytest.mark.parametrize("which", ["grad of one, weight of the other", "overlapping rows", "weight in a longer gradient",
+                                   "momentum under bf16 weight"])
+def test_muon_refuses_memory_that_is_written_and_used_elsewhere(which):
+    flat = torch.zeros(64)
+    p, g, m, lp = [Z(4, 4), Z(4, 4)], [Z(4, 4), Z(4, 4)], [Z(4, 4), Z(4, 4)], [None, None]
+    if which.startswith("grad"):
+        g[0] = p[1]
+    elif which.startswith("overlapping"):
+        p[0], m[1] = flat[:16].view(4, 4), flat[12:28].view(4, 4)
+    elif which.startswith("weight"):
+        p[0], g[0], m[0] = flat[8:24].view(4, 4), flat[:16].view(4, 4), Z(4, 4)
+    else:
+        m[0] = flat[:16].view(4, 4)
+        lp[1] = flat.view(torch.bfloat16)[16:32].view(4, 4)
+    with pytest.raises(ValueError, match="shares its memory"):
+        K.muon_step(p, g, m, lp, lr=0.1)
+
+
+def test_muon_gradients_may_be_one_tensor():
+    """Only read: refused for the device alone here."""
+    g = Z(4, 4)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        K.muon_step([Z(4, 4), Z(4, 4)], [g, g], [Z(4, 4), Z(4, 4)], [None, None], lr=0.1)
+
+
 def test_segments():
     assert [K.ns_segments(n) for n in (1, 2, 3, 4, 5, 6, 7, 10)] == [[1], [2], [3], [2, 2], [3, 2], [3, 3], [3, 2, 2], [3, 3, 2, 2]]
 
