@@ -140,7 +140,8 @@ def ptr(t):
 
 
 def stream():
-    return c_void_p(torch.cuda.current_stream().cuda_stream)
+    # the current stream's handle alone: torch.cuda.current_stream() builds a Stream object around it (3 us a call, 0.3 so)
+    return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def check(rc, what):
