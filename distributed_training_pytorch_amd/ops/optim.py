@@ -320,6 +320,10 @@ class FusedMuon(_FusedBase):
         for i, _, _, at in self._aux:
             self.state[self.arena.params[i]]["exp_avg_sq"] = self._exp_avg_sq_view(i, at)
 
+    def state_dict(self):
+        self._steps = int(self._step_device)      # a step in a graph of the caller's own moves the device's count alone
+        return super().state_dict()
+
     def load_state_dict(self, state_dict):
         mine = {i for i, _, _, _ in self._aux}
         for i, st in state_dict.get("state", {}).items():

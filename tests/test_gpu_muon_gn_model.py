@@ -143,6 +143,31 @@ def test_captured_step_equals_eager_step():
     assert opt._steps == 7 and int(opt._step_device) == 7
 
 
+def test_a_graph_of_the_callers_own_counts_its_steps():
+    """optimizer.step() alone in a graph: each replay equals an eager step with the same gradients, and the snapshot
+    holds the number of steps that ran."""
+    model, opt, crit, x, y = _parts(dropout=0.0)
+    _step(model, opt, crit, x, y)
+    ref, ropt, _, _, _ = _parts(dropout=0.0)
+    ref.load_state_dict(copy.deepcopy(model.state_dict()))
+    ropt.load_state_dict(copy.deepcopy(opt.state_dict()))
+    ropt.zero_grad()
+    crit(ref(x), y).backward()
+    opt.zero_grad()
+    crit(model(x), y).backward()
+    assert torch.equal(model.param_arena.flat_grad, ref.param_arena.flat_grad)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        opt.step()
+    for k in range(3):
+        g.replay()
+        ropt.step()
+        torch.cuda.synchronize()
+        assert torch.equal(model.param_arena.flat_master, ref.param_arena.flat_master), k
+    assert opt.state_dict()["fused_steps"] == ropt.state_dict()["fused_steps"] == 4
+
+
 def test_resume_continues_bit_for_bit():
     model, opt, crit, x, y = _parts(dropout=0.0)
     for _ in range(2):
