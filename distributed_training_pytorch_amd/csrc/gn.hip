@@ -419,7 +419,7 @@ __global__ __launch_bounds__(NT) void gn_slab_bwd_kernel(const void* __restrict_
 // Any size: partial sums over pieces of an image, a fold, and a second pass over the data.
 // A block's threads stand in rows of min(C / VEC, 256) columns; a thread keeps its column, so its channels'
 // parameters stay in registers.
-// Bound by HBM and the last-level cache: 64x224x224x64 bf16 forward 73 + 5 + 129 us, 6.0 TB/s; backward 122 + 6 + 209 + 5.
+// Bound by HBM and the last-level cache: 64x224x224x64 bf16 forward 73 + 5 + 129 us, 6.0 TB/s; backward 122 + 6 + 209.
 constexpr int GN_T = 256;
 
 // Both passes over data that does not stay in the caches as a whole: the first reads from the front and the second from the
@@ -620,18 +620,23 @@ __global__ __launch_bounds__(GN_FOLD) void gn_bwd_fold_kernel(const float* __res
   }
 }
 
-// dgamma / dbeta: the images' channel sums [N][2][C], 16 channels a block, 16 strands of images a channel,
+// dgamma / dbeta: the images' channel sums [N][2][C], 16 channels a block of 256 threads, 16 strands of images a channel,
 // summed in f64 in a fixed order; written, or added to what is there (beta_* = 1)
-__global__ __launch_bounds__(256) void gn_dparam_kernel(const float* __restrict__ sums, int N, int C,
-                                                        void* __restrict__ dgamma, void* __restrict__ dbeta, int out_fp32,
-                                                        float beta_g, float beta_b) {
+struct GnParams {
+  const float* sums;
+  void *dgamma, *dbeta;
+  int N, C, out_fp32;
+  float beta_g, beta_b;
+};
+
+DTP_DEVINL void param_sums(const GnParams& p, const int block) {
   __shared__ double red[2][16][16];
-  const int ci = threadIdx.x & 15, part = threadIdx.x >> 4, c = blockIdx.x * 16 + ci;
+  const int ci = threadIdx.x & 15, part = threadIdx.x >> 4, c = block * 16 + ci, C = p.C;
   double a = 0.0, b = 0.0;
   if (c < C) {
-    for (int n = part; n < N; n += 16) {
-      a += (double)sums[((size_t)n * 2) * C + c];
-      b += (double)sums[((size_t)n * 2 + 1) * C + c];
+    for (int n = part; n < p.N; n += 16) {
+      a += (double)p.sums[((size_t)n * 2) * C + c];
+      b += (double)p.sums[((size_t)n * 2 + 1) * C + c];
     }
   }
   red[0][part][ci] = a;
@@ -640,23 +645,31 @@ __global__ __launch_bounds__(256) void gn_dparam_kernel(const float* __restrict_
   if (part != 0 || c >= C) return;
   a = b = 0.0;
   for (int k = 0; k < 16; ++k) { a += red[0][k][ci]; b += red[1][k][ci]; }
-  if (out_fp32) {
-    float* dg = (float*)dgamma; float* db = (float*)dbeta;
-    dg[c] = (beta_g != 0.f ? beta_g * dg[c] : 0.f) + (float)b;
-    db[c] = (beta_b != 0.f ? beta_b * db[c] : 0.f) + (float)a;
+  if (p.out_fp32) {
+    float* dg = (float*)p.dgamma; float* db = (float*)p.dbeta;
+    dg[c] = (p.beta_g != 0.f ? p.beta_g * dg[c] : 0.f) + (float)b;
+    db[c] = (p.beta_b != 0.f ? p.beta_b * db[c] : 0.f) + (float)a;
   } else {
-    bf16_t* dg = (bf16_t*)dgamma; bf16_t* db = (bf16_t*)dbeta;
-    dg[c] = f32_to_bf16((beta_g != 0.f ? beta_g * bf16_to_f32(dg[c]) : 0.f) + (float)b);
-    db[c] = f32_to_bf16((beta_b != 0.f ? beta_b * bf16_to_f32(db[c]) : 0.f) + (float)a);
+    bf16_t* dg = (bf16_t*)p.dgamma; bf16_t* db = (bf16_t*)p.dbeta;
+    dg[c] = f32_to_bf16((p.beta_g != 0.f ? p.beta_g * bf16_to_f32(dg[c]) : 0.f) + (float)b);
+    db[c] = f32_to_bf16((p.beta_b != 0.f ? p.beta_b * bf16_to_f32(db[c]) : 0.f) + (float)a);
   }
 }
+__global__ __launch_bounds__(256) void gn_dparam_kernel(const GnParams p) { param_sums(p, blockIdx.x); }
 
+// Second pass; backward: its first `lead` blocks fold the parameters' gradients (64x56x56x256 87 us; in a launch of
+// their own 92)
 template <class T, int VEC, int BWD>
 __global__ __launch_bounds__(GN_T) void gn_apply_kernel(const void* __restrict__ x_, const void* __restrict__ dy_,
                                                         const float* __restrict__ gamma, const float* __restrict__ beta,
                                                         const float* __restrict__ stats, const float* __restrict__ coef,
-                                                        void* __restrict__ out_, const GnShape s, const int act) {
+                                                        void* __restrict__ out_, const GnShape s, const int act,
+                                                        const int lead, const GnParams params) {
   typedef typename Pack<T, VEC>::word word;
+  if (BWD && (int)blockIdx.x < lead) {
+    param_sums(params, blockIdx.x);
+    return;
+  }
   const int block = gridDim.x - 1 - blockIdx.x;      // the pieces read last first
   const int n = block / s.chunks, chunk = block - n * s.chunks;
   const int r0 = chunk * s.rows, r1 = min(s.HW, r0 + s.rows);
@@ -795,7 +808,7 @@ int slab_groups(const GnShape& s, int vec, int elem, int bwd, int& threads) {
 bool grids_fit(const GnShape& s, int vec, int elem, int bwd) {
   int nt;
   const int sg = slab_groups(s, vec, elem, bwd, nt);
-  long most = sg ? (long)s.N * ((s.G + sg - 1) / sg) * nt : (long)s.N * s.chunks * GN_T;
+  long most = sg ? (long)s.N * ((s.G + sg - 1) / sg) * nt : ((long)s.N * s.chunks + 256) * GN_T;
   if (!sg) most = max(most, bwd ? (long)s.N * GN_FOLD : ((long)s.N * s.G + 3) / 4 * 256);
   return most < 1L << 32;
 }
@@ -824,7 +837,7 @@ int gn_run_fwd(const void* x, const float* gamma, const float* beta, void* y, fl
   const dim3 grid(s.N * s.chunks);
   hipLaunchKernelGGL((gn_partial_kernel<T, VEC, 0>), grid, dim3(GN_T), lds, st, x, nullptr, gamma, beta, nullptr, ws, s, act);
   hipLaunchKernelGGL((gn_stats_kernel<T, VEC>), dim3((unsigned)(((long)s.N * s.G + 3) / 4)), dim3(256), 0, st, x, ws, stats, s, eps);
-  hipLaunchKernelGGL((gn_apply_kernel<T, VEC, 0>), grid, dim3(GN_T), 0, st, x, nullptr, gamma, beta, stats, nullptr, y, s, act);
+  hipLaunchKernelGGL((gn_apply_kernel<T, VEC, 0>), grid, dim3(GN_T), 0, st, x, nullptr, gamma, beta, stats, nullptr, y, s, act, 0, GnParams{});
   return DTP_CHECK_LAUNCH();
 }
 
@@ -835,6 +848,8 @@ int gn_run_bwd(const void* x, const void* dy, const float* gamma, const float* b
   const size_t np = partial_floats(s, 1), ns = (size_t)s.N * 2 * s.C, nc = (size_t)s.N * s.G * 2;
   if (ws_floats < ns) return -12;
   float *sums = ws, *coef = sums + ns, *partial = coef + nc;
+  const int lead = (s.C + 15) / 16;
+  const GnParams params = {sums, dgamma, dbeta, s.N, s.C, out_fp32, beta_g, beta_b};
   int NT = 0;
   GnSlab sl;
   sl.SG = slab_groups(s, VEC, T::size, 1, NT);
@@ -844,8 +859,7 @@ int gn_run_bwd(const void* x, const void* dy, const float* gamma, const float* b
     const dim3 g((unsigned)((long)s.N * sl.slabs));
     if (NT == 256) hipLaunchKernelGGL((gn_slab_bwd_kernel<T, VEC, 256, 8>), g, dim3(256), slds, st, x, dy, gamma, beta, stats, dx, sums, s, sl, act);
     else hipLaunchKernelGGL((gn_slab_bwd_kernel<T, VEC, 512, 16>), g, dim3(512), slds, st, x, dy, gamma, beta, stats, dx, sums, s, sl, act);
-    hipLaunchKernelGGL(gn_dparam_kernel, dim3((s.C + 15) / 16), dim3(256), 0, st, sums, s.N, s.C, dgamma, dbeta, out_fp32,
-                       beta_g, beta_b);
+    hipLaunchKernelGGL(gn_dparam_kernel, dim3(lead), dim3(256), 0, st, params);
     return DTP_CHECK_LAUNCH();
   }
   if (ws_floats < np + ns + nc) return -12;
@@ -853,9 +867,8 @@ int gn_run_bwd(const void* x, const void* dy, const float* gamma, const float* b
   const dim3 grid(s.N * s.chunks);
   hipLaunchKernelGGL((gn_partial_kernel<T, VEC, 1>), grid, dim3(GN_T), lds, st, x, dy, gamma, beta, stats, partial, s, act);
   hipLaunchKernelGGL(gn_bwd_fold_kernel, dim3(s.N), dim3(GN_FOLD), (size_t)2 * s.C * sizeof(float), st, partial, gamma, sums, coef, s);
-  hipLaunchKernelGGL((gn_apply_kernel<T, VEC, 1>), grid, dim3(GN_T), 0, st, x, dy, gamma, beta, stats, coef, dx, s, act);
-  hipLaunchKernelGGL(gn_dparam_kernel, dim3((s.C + 15) / 16), dim3(256), 0, st, sums, s.N, s.C, dgamma, dbeta, out_fp32,
-                     beta_g, beta_b);
+  hipLaunchKernelGGL((gn_apply_kernel<T, VEC, 1>), dim3(grid.x + lead), dim3(GN_T), 0, st, x, dy, gamma, beta, stats, coef, dx, s, act,
+                     lead, params);
   return DTP_CHECK_LAUNCH();
 }
 

@@ -964,33 +964,43 @@ GN_DTYPES = {BF16: 0, torch.float16: 1, torch.float32: 2}
 GN_ACTS = {"none": 0, "relu": 1, "silu": 2}
 
 
+_HERE = _contextlib.nullcontext()
+
+
 def _on_device_of(t):
     """The launch goes to the current stream of the tensors' own device, whatever device is current."""
-    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else _contextlib.nullcontext()
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+@_functools.lru_cache(maxsize=256)
+def _gn_shape(shape, groups):
+    if len(shape) < 2:
+        raise ValueError("group norm: x must be [N, ..., C], got %s" % (tuple(shape),))
+    N, C, G = shape[0], shape[-1], int(groups)
+    if G < 1 or C < 1 or C % G or C > 4096:
+        raise ValueError("group norm: %d channels in %d groups (channels must be a multiple of groups, at most 4096)" % (C, G))
+    HW = 1
+    for d in shape[1:-1]:
+        HW *= d
+    if HW == 0 and N > 0:
+        raise ValueError("group norm: no values to normalise in %s" % (tuple(shape),))
+    if HW * C >= 2 ** 31 - 1 or N * HW >= 2 ** 31 - 1:
+        raise ValueError("group norm: %s is too large (2^31 values an image, 2^31 pixels)" % (tuple(shape),))
+    return N, HW, C, G
 
 
 def _gn_check(x, groups, act, *vecs):
     if not torch.is_tensor(x) or x.dtype not in GN_DTYPES:
         raise ValueError("group norm: x must be a bf16, f16 or f32 tensor")
-    if x.dim() < 2:
-        raise ValueError("group norm: x must be [N, ..., C], got %s" % (tuple(x.shape),))
     if act not in GN_ACTS:
         raise ValueError("group norm: act must be one of %s, got %r" % (sorted(GN_ACTS), act))
-    N, C, G = x.shape[0], x.shape[-1], int(groups)
-    if G < 1 or C < 1 or C % G or C > 4096:
-        raise ValueError("group norm: %d channels in %d groups (channels must be a multiple of groups, at most 4096)" % (C, G))
-    HW = 1
-    for d in x.shape[1:-1]:
-        HW *= d
-    if HW == 0 and N > 0:
-        raise ValueError("group norm: no values to normalise in %s" % (tuple(x.shape),))
-    if HW * C >= 2 ** 31 - 1 or N * HW >= 2 ** 31 - 1:
-        raise ValueError("group norm: %s is too large (2^31 values an image, 2^31 pixels)" % (tuple(x.shape),))
+    dims = _gn_shape(x.shape, groups)
+    C, device = dims[2], x.device
     for v in vecs:
-        if v.dtype != torch.float32 or not v.is_contiguous() or v.numel() != C or v.device != x.device:
+        if v.dtype != torch.float32 or v.numel() != C or v.device != device or not v.is_contiguous():
             raise ValueError("group norm: gamma / beta must be contiguous f32 [C] on x's device")
     _need(x, x.dtype, "x")
-    return N, HW, C, G
+    return dims
 
 
 @_functools.lru_cache(maxsize=256)
@@ -1008,7 +1018,7 @@ def gn_fwd(x, gamma, beta, groups, eps=1e-5, act="relu"):
     for :func:`gn_bwd`."""
     N, HW, C, G = _gn_check(x, groups, act, gamma, beta)
     y = torch.empty_like(x)
-    stats = torch.empty((N, G, 2), dtype=torch.float32, device=x.device)
+    stats = gamma.new_empty((N, G, 2))
     if N == 0:
         return y, stats
     dt = GN_DTYPES[x.dtype]
@@ -1017,9 +1027,9 @@ def gn_fwd(x, gamma, beta, groups, eps=1e-5, act="relu"):
         # scratch of this call alone (the caching allocator's, so a captured graph keeps its own): calls on two
         # streams, or two graphs, share nothing
         n = _gn_workspace(N, HW, C, G, dt, 0)
-        ws = torch.empty(n, dtype=torch.float32, device=x.device) if n else None
-        check(lib.dtp_gn_fwd(ptr(x), ptr(gamma), ptr(beta), ptr(y), ptr(stats), ptr(ws), n, N, HW, C, G, dt,
-                             GN_ACTS[act], float(eps), stream()), "gn_fwd")
+        ws = gamma.new_empty(n) if n else None
+        check(lib.dtp_gn_fwd(x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), y.data_ptr(), stats.data_ptr(), ptr(ws), n,
+                             N, HW, C, G, dt, GN_ACTS[act], float(eps), stream()), "gn_fwd")
     return y, stats
 
 
@@ -1030,14 +1040,14 @@ def gn_bwd(x, dy, gamma, beta, stats, groups, dgamma, dbeta, act="relu", beta_g=
         raise ValueError("gn_bwd: dy must have x's shape, type and device")
     N, HW, C, G = _gn_check(x, groups, act, gamma, beta)
     _need(dy, x.dtype, "dy")
-    if stats.dtype != torch.float32 or tuple(stats.shape) != (N, G, 2) or not stats.is_contiguous() or stats.device != x.device:
+    if stats.dtype != torch.float32 or stats.shape != (N, G, 2) or not stats.is_contiguous() or stats.device != x.device:
         raise ValueError("gn_bwd: stats must be gn_fwd's [N, groups, 2] f32")
     if dgamma.dtype != dbeta.dtype or dgamma.dtype not in (torch.float32, BF16) or dgamma.numel() != C \
             or dbeta.numel() != C or not dgamma.is_contiguous() or not dbeta.is_contiguous() \
             or dgamma.device != x.device or dbeta.device != x.device:
         raise ValueError("gn_bwd: dgamma / dbeta must be contiguous [C] of one dtype (f32 / bf16) on x's device")
-    if dgamma.data_ptr() == dbeta.data_ptr():
-        raise ValueError("gn_bwd: dgamma and dbeta share their memory")
+    if len({dgamma.data_ptr(), dbeta.data_ptr()} - {gamma.data_ptr(), beta.data_ptr()}) < 2:
+        raise ValueError("gn_bwd: dgamma and dbeta share their memory with each other or with gamma / beta")
     dx = torch.empty_like(x)
     if N == 0:
         if beta_g == 0.0:
@@ -1048,10 +1058,11 @@ def gn_bwd(x, dy, gamma, beta, stats, groups, dgamma, dbeta, act="relu", beta_g=
     dt = GN_DTYPES[x.dtype]
     lib = _lib.hip()
     with _on_device_of(x):
-        ws = torch.empty(_gn_workspace(N, HW, C, G, dt, 1), dtype=torch.float32, device=x.device)
-        check(lib.dtp_gn_bwd(ptr(x), ptr(dy), ptr(gamma), ptr(beta), ptr(stats), ptr(dx), ptr(dgamma), ptr(dbeta),
-                             int(dgamma.dtype == torch.float32), float(beta_g), float(beta_b), ptr(ws), ws.numel(), N, HW,
-                             C, G, dt, GN_ACTS[act], stream()), "gn_bwd")
+        n = _gn_workspace(N, HW, C, G, dt, 1)
+        ws = gamma.new_empty(n)
+        check(lib.dtp_gn_bwd(x.data_ptr(), dy.data_ptr(), gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(), dx.data_ptr(),
+                             dgamma.data_ptr(), dbeta.data_ptr(), dgamma.dtype == torch.float32, float(beta_g), float(beta_b),
+                             ws.data_ptr(), n, N, HW, C, G, dt, GN_ACTS[act], stream()), "gn_bwd")
     return dx
 
 

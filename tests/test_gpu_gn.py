@@ -270,3 +270,5 @@ def test_gn_bwd_refuses_one_tensor_for_both_parameter_gradients():
     d = torch.zeros(16, device="cuda")
     with pytest.raises(ValueError, match="share their memory"):
         k.gn_bwd(x, dy, gamma, beta, stats, 4, d, d)
+    with pytest.raises(ValueError, match="share their memory"):
+        k.gn_bwd(x, dy, gamma, beta, stats, 4, d, beta)
