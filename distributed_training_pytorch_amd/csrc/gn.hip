@@ -5,12 +5,15 @@
 //   backward   dz = dy * act'(z);  dbeta = sum_{n,hw} dz;  dgamma = sum_{n,hw} dz * xhat
 //              dx = rstd * (gamma*dz - m1 - xhat*m2),  m1 = mean_group(gamma*dz),  m2 = mean_group(gamma*dz*xhat)
 //
-// x, y, dy, dx: bf16, f16 or f32; gamma, beta, statistics and every sum: f32 (folds of partial sums in f64);
-// one rounding, of the result.  Statistics of an image never leave it, so nothing is shared between images but
-// the gamma / beta gradients, which a last kernel sums in a fixed order (no atomics: results repeat bit for bit).
+// x, y, dy, dx: bf16, f16 or f32; gamma, beta, statistics and a thread's sums: f32; one rounding, of the result.
+// Statistics of an image never leave it, so nothing is shared between images but the gamma / beta gradients, which a last
+// kernel sums in a fixed order (no atomics: results repeat bit for bit).
 //
-// Variance: sums of (x - p) and (x - p)^2 with p = the group's first value, so that a mean far from zero does not
-// cancel (E[x^2] - mean^2 in f32 loses mean^2 / var * 6e-8).
+// Variance: every thread takes the mean c of a few values that it holds and M = sum of (x - c)^2 around it; sets of n values
+// meet as  M = sum of M_t + n_t (c_t - mean)^2,  in f64 between threads and pieces.  Nothing but squares is added, so neither
+// a mean far from zero nor a value far from the others cancels: rstd is good to a few units of f32 whatever the data.
+// (Sums around one value of the group, its first: 5e-5 off where that value lies 30 standard deviations from the mean,
+// 2e-3 at 300.  E[x^2] - mean^2 loses mean^2 / var * 6e-8.)
 #include "dtp_common.h"
 
 #include <utility>
@@ -104,10 +107,20 @@ template <class F> DTP_DEVINL void with_act(int act, F&& f) {
   else f(std::integral_constant<int, ACT_NONE>{});
 }
 
+template <int CTRL> DTP_DEVINL float add_turned(float v) {       // v + v of the lane that many places on in its row of 16
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+template <int CTRL> DTP_DEVINL double add_turned(double v) {
+  return v + __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xF, 0xF, true),
+                              __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xF, 0xF, true));
+}
 DTP_DEVINL double wave_reduce_sum_f64(double v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+  v = add_turned<0x121>(v);                          // row_ror:1, 2, 4, 8
+  v = add_turned<0x122>(v);
+  v = add_turned<0x124>(v);
+  v = add_turned<0x128>(v);
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
 }
 
 struct GnShape {
@@ -117,13 +130,12 @@ struct GnShape {
   int once;                  // so many pieces from the front are read past the caches (GN_KEEP)
 };
 
-// The value around which a group's sums are taken: its first one in the image.
-template <class T, int VEC>
-DTP_DEVINL float pivot_of(const typename Pack<T, VEC>::word* xn, int group, int cpg) {
-  float f;
-  Pack<T, 1>::unpack(((const typename Pack<T, 1>::word*)xn)[(size_t)group * cpg], &f);
-  return f;
-}
+// n rows dealt out in turn: how many the k-th of R threads gets
+struct Deal {
+  int each, more;
+  DTP_DEVINL Deal(int n, int R) : each(n / R), more(n - n / R * R) {}
+  DTP_DEVINL int operator()(int k) const { return each + (k < more ? 1 : 0); }
+};
 
 // ---------------------------------------------------------------------------------------------------------
 // Images whose groups fit a workgroup's registers: x is read once and y written once (backward: x and dy read once).
@@ -147,9 +159,6 @@ DTP_DEVINL int column_rows(int TX, int NT, int ty, int R, int& rows) {
   rows = R;
   return ty < R ? ty : -1;
 }
-template <int CTRL> DTP_DEVINL float add_turned(float v) {       // v + v of the lane that many places on in its row of 16
-  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
-}
 DTP_DEVINL float column_sum(float v, int TX) {       // over the lanes l, l + TX, ... of the wave
   if ((TX & (TX - 1)) != 0 || TX > 32) return v;
   if (TX <= 1) v = add_turned<0x121>(v);             // row_ror:1, 2, 4, 8
@@ -169,6 +178,29 @@ template <int VEC> DTP_DEVINL void groups_of(int c, int cpg, int* g) {
   }
 }
 
+// Sums over the u neighbours that make a unit, left in each of them
+template <int VEC> DTP_DEVINL void unit_sums(float* a, int u) {
+  if constexpr (VEC > 1) {
+    if (u >= 2) {
+#pragma unroll
+      for (int e = 0; e < VEC; e += 2) a[e] = a[e + 1] = a[e] + a[e + 1];
+    }
+  }
+  if constexpr (VEC > 2) {
+    if (u >= 4) {
+#pragma unroll
+      for (int e = 0; e < VEC; e += 4) a[e] = a[e + 1] = a[e + 2] = a[e + 3] = a[e] + a[e + 2];
+    }
+  }
+  if constexpr (VEC > 4) {
+    if (u >= 8) {
+      const float t = a[0] + a[4];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) a[e] = t;
+    }
+  }
+}
+
 // f(0), f(1), .. f(N - 1) with the number known where the body is compiled: as a loop, the kept words of some types came to
 // lie in one wide vector, copied at every row's condition (up to 3.5 KB a lane in scratch memory).
 template <class F, int... I> DTP_DEVINL void each_of(F&& f, std::integer_sequence<int, I...>) {
@@ -182,7 +214,7 @@ __global__ __launch_bounds__(NT) void gn_slab_fwd_kernel(const void* __restrict_
                                                          float* __restrict__ stats, const GnShape s, const GnSlab sl,
                                                          const float eps, const int act) {
   typedef typename Pack<T, VEC>::word word;
-  extern __shared__ float sm[];                     // [2][rows][units of a row], then [SG][2] mean, rstd
+  extern __shared__ float sm[];                     // [3][R][units of a row], then [SG][2] mean, rstd
   const int block = xcd_remap(blockIdx.x, gridDim.x);
   const int n = block / sl.slabs, slab = block - n * sl.slabs;
   const int g0 = slab * sl.SG, ng = min(sl.SG, s.G - g0);
@@ -196,14 +228,29 @@ __global__ __launch_bounds__(NT) void gn_slab_fwd_kernel(const void* __restrict_
     const int r = ty + i * R;
     if (ty < R && r < s.HW) w[i] = xn[(size_t)r * s.CV];
   });
-  float p[VEC], a0[VEC], a1[VEC];
-  int gl[VEC];                                      // group within the slab
-  groups_of<VEC>(tx * VEC, s.cpg, gl);
+  // neighbouring channels of one group and thread are one unit of u = gcd(cpg, VEC)
+  int u = 1;
+  if (VEC > 1 && s.cpg % 2 == 0) u = 2;
+  if (VEC > 2 && s.cpg % 4 == 0) u = 4;
+  if (VEC > 4 && s.cpg % 8 == 0) u = 8;
+  const Deal dealt(s.HW, R);
+  const int count = ty < R ? dealt(ty) * u : 0;
+  const float inv = count ? 1.f / (float)count : 0.f;
+  float c[VEC], a0[VEC], a1[VEC];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    p[e] = pivot_of<T, VEC>((const word*)x_ + base, g0 + gl[e], s.cpg);
-    a0[e] = a1[e] = 0.f;
-  }
+  for (int e = 0; e < VEC; ++e) c[e] = a0[e] = a1[e] = 0.f;
+  each<KV>([&](auto i) {
+    const int r = ty + i * R;
+    if (ty < R && r < s.HW) {
+      float f[VEC];
+      Pack<T, VEC>::unpack(w[i], f);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) c[e] += f[e];
+    }
+  });
+  unit_sums<VEC>(c, u);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) c[e] *= inv;        // the thread's mean, or next to it: a0 is what it misses
   each<KV>([&](auto i) {
     const int r = ty + i * R;
     if (ty < R && r < s.HW) {
@@ -211,69 +258,57 @@ __global__ __launch_bounds__(NT) void gn_slab_fwd_kernel(const void* __restrict_
       Pack<T, VEC>::unpack(w[i], f);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float d = f[e] - p[e];
+        const float d = f[e] - c[e];
         a0[e] += d;
         a1[e] = fmaf(d, d, a1[e]);
       }
     }
   });
-  // neighbouring channels of one group and thread are one unit of u = gcd(cpg, VEC)
-  int u = 1;
-  if (VEC > 1 && s.cpg % 2 == 0) {
-    u = 2;
+  unit_sums<VEC>(a0, u);
+  unit_sums<VEC>(a1, u);
+  const int nu = VEC / u, m = s.cpg / u, row = TX * nu, plane = R * row;
+  if (ty < R) {
 #pragma unroll
-    for (int e = 0; e + 1 < VEC; e += 2) { a0[e] += a0[e + 1]; a1[e] += a1[e + 1]; }
-    if (VEC > 2 && s.cpg % 4 == 0) {
-      u = 4;
-#pragma unroll
-      for (int e = 0; e + 2 < VEC; e += 4) { a0[e] += a0[e + 2]; a1[e] += a1[e + 2]; }
-      if (VEC > 4 && s.cpg % 8 == 0) {
-        u = 8;
-        a0[0] += a0[VEC / 2];
-        a1[0] += a1[VEC / 2];
-      }
-    }
-  }
-  const int nu = VEC / u, m = s.cpg / u, row = TX * nu;
-  int rows;
-  const int mine = column_rows(TX, NT, ty, R, rows);
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    if (e % u == 0) {
-      const float b0 = column_sum(a0[e], TX), b1 = column_sum(a1[e], TX);
-      if (mine >= 0) {
-        sm[mine * row + tx * nu + e / u] = b0;
-        sm[(rows + mine) * row + tx * nu + e / u] = b1;
+    for (int e = 0; e < VEC; ++e) {
+      if (e % u == 0) {
+        const int j = ty * row + tx * nu + e / u;
+        const float miss = a0[e] * inv;
+        sm[j] = c[e];
+        sm[plane + j] = miss;
+        sm[2 * plane + j] = fmaf(-a0[e], miss, a1[e]);
       }
     }
   }
   __syncthreads();
-  float* ms = sm + 2 * rows * row;
+  float* ms = sm + 3 * plane;
   const int lane = threadIdx.x & 63;
+  const double mm = (double)s.HW * s.cpg;
   for (int g = threadIdx.x >> 6; g < ng; g += NT / 64) {
-    float b0 = 0.f, b1 = 0.f;
-    for (int i = lane; i < rows * m; i += 64) {
+    double a = 0.0, v = 0.0;
+    for (int i = lane; i < R * m; i += 64) {
       const int r = i / m, j = r * row + g * m + i - r * m;
-      b0 += sm[j];
-      b1 += sm[rows * row + j];
+      a += (double)(dealt(r) * u) * ((double)sm[j] + (double)sm[plane + j]);
     }
-    b0 = wave_reduce_sum(b0);
-    b1 = wave_reduce_sum(b1);
+    const double mean = wave_reduce_sum_f64(a) / mm;
+    for (int i = lane; i < R * m; i += 64) {
+      const int r = i / m, j = r * row + g * m + i - r * m;
+      const double d = ((double)sm[j] + (double)sm[plane + j]) - mean;
+      v += (double)sm[2 * plane + j] + (double)(dealt(r) * u) * d * d;
+    }
+    v = wave_reduce_sum_f64(v);
     if (lane == 0) {
-      const double pv = (double)pivot_of<T, VEC>((const word*)x_ + base, g0 + g, s.cpg), mm = (double)s.HW * s.cpg;
-      const double d = (double)b0 / mm;
-      double var = (double)b1 / mm - d * d;
-      if (var < 0.0) var = 0.0;
-      const float mean = (float)(pv + d), rstd = (float)(1.0 / sqrt(var + (double)eps));
-      ms[2 * g] = mean;
+      const float rstd = (float)(1.0 / sqrt(v / mm + (double)eps));
+      ms[2 * g] = (float)mean;
       ms[2 * g + 1] = rstd;
       float* o = stats + ((size_t)n * s.G + g0 + g) * 2;
-      o[0] = mean;
+      o[0] = (float)mean;
       o[1] = rstd;
     }
   }
   __syncthreads();
   float mu[VEC], rs[VEC], ga[VEC], be[VEC];
+  int gl[VEC];                                      // group within the slab
+  groups_of<VEC>(tx * VEC, s.cpg, gl);
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
     mu[e] = ms[2 * gl[e]];
@@ -436,17 +471,22 @@ template <bool ONCE, class W> DTP_DEVINL W load_word(const W* p) {
   else return *p;
 }
 
-// BWD 0: per group (sum (x-p), sum (x-p)^2) -> partial [N][chunks][G][2]
-// BWD 1: per channel (sum dz, sum dz*xhat)  -> partial [N][chunks][2][C]
+// Forward: a thread takes its rows in runs of eight: their mean, their squares around it, and both join what it has (the
+// formula at the head).  All of it relative to the mean of its first run, so that a large common mean costs no bits.
+constexpr int GN_RUN = 8;
+
+// BWD 0: per group of the piece its mean (as hi + lo) and M, the sum of squares around it -> partial [N][chunks][G][3]
+// BWD 1: per channel (sum dz, sum dz*xhat) -> partial [N][chunks][2][C]
 template <class T, int VEC, int BWD>
 __global__ __launch_bounds__(GN_T) void gn_partial_kernel(const void* __restrict__ x_, const void* __restrict__ dy_,
                                                           const float* __restrict__ gamma, const float* __restrict__ beta,
                                                           const float* __restrict__ stats, float* __restrict__ partial,
                                                           const GnShape s, const int act) {
   typedef typename Pack<T, VEC>::word word;
-  extern __shared__ float sm[];                     // [2][C] channel sums, then [2][GN_T * VEC] thread sums
-  float* chs = sm;
-  float* thr = sm + 2 * s.C;
+  extern __shared__ float sm[];                     // [2 + (BWD == 0)][GN_T * VEC] the threads'; BWD 0: channels' means (f64), M
+  float* thr = sm;
+  double* chm = (double*)(sm + 3 * GN_T * VEC);
+  float* chv = (float*)(chm + s.C);
   const int n = blockIdx.x / s.chunks, chunk = blockIdx.x - n * s.chunks;
   const int r0 = chunk * s.rows, r1 = min(s.HW, r0 + s.rows);
   const word* xn = (const word*)x_ + (size_t)n * s.HW * s.CV;
@@ -456,32 +496,27 @@ __global__ __launch_bounds__(GN_T) void gn_partial_kernel(const void* __restrict
   for (int cb = 0; cb < s.CV; cb += TX) {
     const int cv = cb + tx;
     const bool on = ty < R && cv < s.CV;
-    float a0[VEC], a1[VEC];
+    float p[VEC], a0[VEC], a1[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) a0[e] = a1[e] = 0.f;
+    for (int e = 0; e < VEC; ++e) p[e] = a0[e] = a1[e] = 0.f;
     if (on) {
-      float p[VEC], rs[VEC], ga[VEC], be[VEC];
+      if constexpr (BWD) {
+        float rs[VEC], ga[VEC], be[VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const int c = cv * VEC + e, g = c / s.cpg;
-        if (BWD) {
+        for (int e = 0; e < VEC; ++e) {
+          const int c = cv * VEC + e, g = c / s.cpg;
           p[e] = stats[((size_t)n * s.G + g) * 2];
           rs[e] = stats[((size_t)n * s.G + g) * 2 + 1];
           ga[e] = gamma[c];
           be[e] = beta[c];
-        } else {
-          p[e] = pivot_of<T, VEC>(xn, g, s.cpg);
         }
-      }
-      const auto rows = [&](auto once, auto which) {
-        constexpr bool ONCE = decltype(once)::value;
-        constexpr int ACT = decltype(which)::value;
+        const auto rows = [&](auto once, auto which) {
+          constexpr bool ONCE = decltype(once)::value;
+          constexpr int ACT = decltype(which)::value;
 #pragma unroll 4
-        for (int r = r0 + ty; r < r1; r += R) {
-          float f[VEC];
-          Pack<T, VEC>::unpack(load_word<ONCE>(xn + (size_t)r * s.CV + cv), f);
-          if (BWD) {
-            float d[VEC];
+          for (int r = r0 + ty; r < r1; r += R) {
+            float f[VEC], d[VEC];
+            Pack<T, VEC>::unpack(load_word<ONCE>(xn + (size_t)r * s.CV + cv), f);
             Pack<T, VEC>::unpack(load_word<ONCE>(dn + (size_t)r * s.CV + cv), d);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
@@ -490,34 +525,104 @@ __global__ __launch_bounds__(GN_T) void gn_partial_kernel(const void* __restrict
               a0[e] += dz;
               a1[e] = fmaf(dz, xh, a1[e]);
             }
-          } else {
+          }
+        };
+        with_act(act, [&](auto which) {
+          if ((int)blockIdx.x < s.once) rows(std::true_type{}, which);
+          else rows(std::false_type{}, which);
+        });
+      } else {
+        // p: mean of this thread's first run, a0: of all its values less that, a1: M
+        const auto rows = [&](auto once) {
+          constexpr bool ONCE = decltype(once)::value;
+          int r = r0 + ty;
+          float have = 0.f;
+          for (; r1 - r > (GN_RUN - 1) * R; r += GN_RUN * R) {
+            word w[GN_RUN];
+#pragma unroll
+            for (int k = 0; k < GN_RUN; ++k) w[k] = load_word<ONCE>(xn + (size_t)(r + k * R) * s.CV + cv);
+            float f[GN_RUN][VEC];
+#pragma unroll
+            for (int k = 0; k < GN_RUN; ++k) Pack<T, VEC>::unpack(w[k], f[k]);
+            if (have == 0.f) {
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) {
+                p[e] = 0.f;
+#pragma unroll
+                for (int k = 0; k < GN_RUN; ++k) p[e] = fmaf(f[k][e], 1.f / GN_RUN, p[e]);
+              }
+            }
+            const float all = have + GN_RUN, part = GN_RUN / all, both = have * part;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-              const float d = f[e] - p[e];
-              a0[e] += d;
-              a1[e] = fmaf(d, d, a1[e]);
+              float c = 0.f, q = 0.f;
+#pragma unroll
+              for (int k = 0; k < GN_RUN; ++k) {
+                f[k][e] -= p[e];
+                c += f[k][e];
+              }
+              c *= 1.f / GN_RUN;
+#pragma unroll
+              for (int k = 0; k < GN_RUN; ++k) {
+                const float d = f[k][e] - c;
+                q = fmaf(d, d, q);
+              }
+              const float d = c - a0[e];
+              a0[e] = fmaf(d, part, a0[e]);
+              a1[e] += fmaf(d * d, both, q);
             }
+            have = all;
           }
-        }
-      };
-      with_act(BWD ? act : ACT_NONE, [&](auto which) {
-        if ((int)blockIdx.x < s.once) rows(std::true_type{}, which);
-        else rows(std::false_type{}, which);
-      });
+          for (; r < r1; r += R) {
+            float f[VEC];
+            Pack<T, VEC>::unpack(load_word<ONCE>(xn + (size_t)r * s.CV + cv), f);
+            const float all = have + 1.f, part = 1.f / all, both = have * part;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              if (have == 0.f) p[e] = f[e];
+              const float d = (f[e] - p[e]) - a0[e];
+              a0[e] = fmaf(d, part, a0[e]);
+              a1[e] = fmaf(d * d, both, a1[e]);
+            }
+            have = all;
+          }
+        };
+        if ((int)blockIdx.x < s.once) rows(std::true_type{});
+        else rows(std::false_type{});
+      }
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         thr[(ty * TX + tx) * VEC + e] = a0[e];
         thr[GN_T * VEC + (ty * TX + tx) * VEC + e] = a1[e];
+        if (!BWD) thr[2 * GN_T * VEC + (ty * TX + tx) * VEC + e] = p[e];
       }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * TX * VEC; i += GN_T) {
-      const int which = i / (TX * VEC), j = i - which * TX * VEC, c = cb * VEC + j;
-      if (c < s.C) {
-        float t = 0.f;
-        for (int k = 0; k < R; ++k) t += thr[which * GN_T * VEC + k * TX * VEC + j];
-        if (BWD) partial[(((size_t)n * s.chunks + chunk) * 2 + which) * s.C + c] = t;
-        else chs[which * s.C + c] = t;
+    if constexpr (BWD) {
+      for (int i = threadIdx.x; i < 2 * TX * VEC; i += GN_T) {
+        const int which = i / (TX * VEC), j = i - which * TX * VEC, c = cb * VEC + j;
+        if (c < s.C) {
+          float t = 0.f;
+          for (int k = 0; k < R; ++k) t += thr[which * GN_T * VEC + k * TX * VEC + j];
+          partial[(((size_t)n * s.chunks + chunk) * 2 + which) * s.C + c] = t;
+        }
+      }
+    } else {
+      for (int j = threadIdx.x; j < TX * VEC; j += GN_T) {
+        const int c = cb * VEC + j, len = r1 - r0;
+        if (c < s.C) {
+          const Deal dealt(len, R);
+          const auto mean_of = [&](int k) { return (double)thr[2 * GN_T * VEC + k * TX * VEC + j] + (double)thr[k * TX * VEC + j]; };
+          double a = 0.0, v = 0.0;
+          for (int k = 0; k < R; ++k) a += (double)dealt(k) * mean_of(k);
+          a /= (double)len;
+          for (int k = 0; k < R; ++k) {
+            const double d = mean_of(k) - a;
+            v += (double)thr[GN_T * VEC + k * TX * VEC + j] + (double)dealt(k) * d * d;
+          }
+          chm[c] = a;
+          chv[c] = (float)v;
+        }
       }
     }
     __syncthreads();
@@ -525,46 +630,47 @@ __global__ __launch_bounds__(GN_T) void gn_partial_kernel(const void* __restrict
   if (!BWD) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     for (int g = wave; g < s.G; g += GN_T / 64) {
-      float u = 0.f, v = 0.f;
+      double a = 0.0, v = 0.0;
+      for (int c = lane; c < s.cpg; c += 64) a += chm[g * s.cpg + c];
+      a = wave_reduce_sum_f64(a) / (double)s.cpg;
       for (int c = lane; c < s.cpg; c += 64) {
-        u += chs[g * s.cpg + c];
-        v += chs[s.C + g * s.cpg + c];
+        const double d = chm[g * s.cpg + c] - a;
+        v += (double)chv[g * s.cpg + c] + (double)(r1 - r0) * d * d;
       }
-      u = wave_reduce_sum(u);
-      v = wave_reduce_sum(v);
+      v = wave_reduce_sum_f64(v);
       if (lane == 0) {
-        float* o = partial + (((size_t)n * s.chunks + chunk) * s.G + g) * 2;
-        o[0] = u;
-        o[1] = v;
+        float* o = partial + (((size_t)n * s.chunks + chunk) * s.G + g) * 3;
+        o[0] = (float)a;
+        o[1] = (float)(a - (double)(float)a);
+        o[2] = (float)v;
       }
     }
   }
 }
 
-// mean and rstd of (image, group) from its pieces' sums: one wave each
-template <class T, int VEC>
-__global__ __launch_bounds__(256) void gn_stats_kernel(const void* __restrict__ x_, const float* __restrict__ partial,
-                                                       float* __restrict__ stats, const GnShape s, const float eps) {
+// mean and rstd of (image, group) from its pieces: one wave each
+__global__ __launch_bounds__(256) void gn_stats_kernel(const float* __restrict__ partial, float* __restrict__ stats,
+                                                       const GnShape s, const float eps) {
   const long idx = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (idx >= (long)s.N * s.G) return;
   const int n = (int)(idx / s.G), g = (int)(idx - (long)n * s.G);
-  double u = 0.0, v = 0.0;
+  const float* pn = partial + ((size_t)n * s.chunks * s.G + g) * 3;
+  double a = 0.0, v = 0.0;
   for (int k = lane; k < s.chunks; k += 64) {
-    const float* o = partial + (((size_t)n * s.chunks + k) * s.G + g) * 2;
-    u += (double)o[0];
-    v += (double)o[1];
+    const float* o = pn + (size_t)k * s.G * 3;
+    a += (double)min(s.rows, s.HW - k * s.rows) * ((double)o[0] + (double)o[1]);
   }
-  u = wave_reduce_sum_f64(u);
+  a = wave_reduce_sum_f64(a) / (double)s.HW;
+  for (int k = lane; k < s.chunks; k += 64) {
+    const float* o = pn + (size_t)k * s.G * 3;
+    const double d = ((double)o[0] + (double)o[1]) - a;
+    v += (double)o[2] + (double)min(s.rows, s.HW - k * s.rows) * (double)s.cpg * d * d;
+  }
   v = wave_reduce_sum_f64(v);
   if (lane == 0) {
-    typedef typename Pack<T, VEC>::word word;
-    const double p = (double)pivot_of<T, VEC>((const word*)x_ + (size_t)n * s.HW * s.CV, g, s.cpg);
-    const double m = (double)s.HW * s.cpg, d = u / m;
-    double var = v / m - d * d;
-    if (var < 0.0) var = 0.0;
-    stats[idx * 2] = (float)(p + d);
-    stats[idx * 2 + 1] = (float)(1.0 / sqrt(var + (double)eps));
+    stats[idx * 2] = (float)a;
+    stats[idx * 2 + 1] = (float)(1.0 / sqrt(v / ((double)s.HW * s.cpg) + (double)eps));
   }
 }
 
@@ -755,7 +861,7 @@ int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 // LDS of a slab kernel (a slab may be the image's last, with fewer groups: any number of columns has its place)
 size_t slab_lds(const GnShape& s, int vec, int sg, int nt, int bwd) {
-  const size_t row = (size_t)2 * nt * (bwd ? vec : vec / gcd(s.cpg, vec));
+  const size_t row = (size_t)nt * (bwd ? 2 * vec : 3 * (vec / gcd(s.cpg, vec)));
   return (row + (bwd ? (size_t)2 * sg * s.cpg : 0) + 2 * (size_t)sg) * sizeof(float);
 }
 
@@ -814,7 +920,7 @@ bool grids_fit(const GnShape& s, int vec, int elem, int bwd) {
 }
 
 size_t partial_floats(const GnShape& s, int bwd) {
-  return bwd ? (size_t)s.N * s.chunks * 2 * s.C : (size_t)s.N * s.chunks * s.G * 2;
+  return bwd ? (size_t)s.N * s.chunks * 2 * s.C : (size_t)s.N * s.chunks * s.G * 3;
 }
 
 template <class T, int VEC>
@@ -833,10 +939,13 @@ int gn_run_fwd(const void* x, const float* gamma, const float* beta, void* y, fl
     return DTP_CHECK_LAUNCH();
   }
   if (ws_floats < partial_floats(s, 0)) return -12;
-  const size_t lds = (size_t)(2 * s.C + 2 * GN_T * VEC) * sizeof(float);
+  const size_t lds = (size_t)(3 * s.C + 3 * GN_T * VEC) * sizeof(float);
+  if (lds > 65536 && hipFuncSetAttribute((const void*)gn_partial_kernel<T, VEC, 0>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)lds) != hipSuccess)
+    return -2;
   const dim3 grid(s.N * s.chunks);
   hipLaunchKernelGGL((gn_partial_kernel<T, VEC, 0>), grid, dim3(GN_T), lds, st, x, nullptr, gamma, beta, nullptr, ws, s, act);
-  hipLaunchKernelGGL((gn_stats_kernel<T, VEC>), dim3((unsigned)(((long)s.N * s.G + 3) / 4)), dim3(256), 0, st, x, ws, stats, s, eps);
+  hipLaunchKernelGGL(gn_stats_kernel, dim3((unsigned)(((long)s.N * s.G + 3) / 4)), dim3(256), 0, st, ws, stats, s, eps);
   hipLaunchKernelGGL((gn_apply_kernel<T, VEC, 0>), grid, dim3(GN_T), 0, st, x, nullptr, gamma, beta, stats, nullptr, y, s, act, 0, GnParams{});
   return DTP_CHECK_LAUNCH();
 }
@@ -863,7 +972,7 @@ int gn_run_bwd(const void* x, const void* dy, const float* gamma, const float* b
     return DTP_CHECK_LAUNCH();
   }
   if (ws_floats < np + ns + nc) return -12;
-  const size_t lds = (size_t)(2 * s.C + 2 * GN_T * VEC) * sizeof(float);
+  const size_t lds = (size_t)(2 * GN_T * VEC) * sizeof(float);
   const dim3 grid(s.N * s.chunks);
   hipLaunchKernelGGL((gn_partial_kernel<T, VEC, 1>), grid, dim3(GN_T), lds, st, x, dy, gamma, beta, stats, partial, s, act);
   hipLaunchKernelGGL(gn_bwd_fold_kernel, dim3(s.N), dim3(GN_FOLD), (size_t)2 * s.C * sizeof(float), st, partial, gamma, sums, coef, s);

@@ -272,3 +272,77 @@ def test_gn_bwd_refuses_one_tensor_for_both_parameter_gradients():
         k.gn_bwd(x, dy, gamma, beta, stats, 4, d, d)
     with pytest.raises(ValueError, match="share their memory"):
         k.gn_bwd(x, dy, gamma, beta, stats, 4, d, beta)
+
+
+def _check_stats(stats, x, groups, name):
+    """Statistics against 64 bits.  U = 2^-24.  A thread's squares: 3 U a term (difference, square), at most 16 additions in
+    one launch; in two passes runs of 8 and one addition a run of at most 16 runs: 24 U in all.  A set's centre is off by
+    2 U of its size, which moves the variance by 2 * 2 U of (centre - mean) * size summed over the sets: the centres
+    deviate as little as the values, so 2 * 2 U times what the largest |x - mean| of a set is to the spread, <= 32 U.  rstd: half
+    of the variance's error, and 2 U of its own: 30 U; twice that is allowed.  The mean: 2 U of a set's centre, 8 U of
+    adding up a set."""
+    mean, rstd, mag = _ref_stats(x, groups, 1e-5)
+    err = ((stats[..., 1].double() - rstd).abs() / rstd).max().item()
+    assert err <= 60 * U, "%s: rstd is %.3g off" % (name, err)
+    err = ((stats[..., 0].double() - mean).abs() / mag).max().item()
+    assert err <= 10 * U, "%s: mean is %.3g of E|x| off" % (name, err)
+
+
+STAT_SHAPES = [((2, 56, 56, 64), 16, False), ((3, 14, 14, 60), 12, False), ((2, 30, 31, 8), 1, False), ((2, 5, 7, 33), 3, False),
+               ((2, 128, 128, 64), 1, True), ((1, 301, 257, 24), 4, True), ((1, 200, 200, 9), 3, True)]
+
+
+@pytest.mark.parametrize("far", [30.0, 300.0, 1e4, 1e6])
+@pytest.mark.parametrize("where", ["first", "last", "corner rows"])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("shape,groups,two_passes", STAT_SHAPES)
+def test_gn_statistics_beside_values_far_from_the_others(shape, groups, two_passes, dtype, where, far):
+    """A group's first value, its last one, or the image's first row and column, `far` standard deviations from the rest:
+    sums around such a value cancel (around the first: 7e-3 of rstd at 1000)."""
+    if dtype == F16 and far > 6e4:
+        far = 6e4
+    k = _k()
+    n, c = shape[0], shape[-1]
+    hw = 1
+    for d in shape[1:-1]:
+        hw *= d
+    dt = k.GN_DTYPES[dtype]
+    slab = k._gn_workspace(n, hw, c, groups, dt, 0) == 0
+    assert slab != two_passes, "the shape does not reach the path that it is here for"
+    g = torch.Generator(device="cuda").manual_seed(11)
+    x = torch.randn(shape, generator=g, device="cuda")
+    first = torch.arange(0, c, c // groups, device="cuda")
+    if where == "first":
+        x[:, 0, 0, first] = far
+    elif where == "last":
+        x[:, -1, -1, first] = -far
+    else:
+        x[:, 0], x[:, :, 0] = far, far
+    x = x.to(dtype)
+    gamma, beta = 1 + 0.3 * torch.randn(c, generator=g, device="cuda"), 0.3 * torch.randn(c, generator=g, device="cuda")
+    y, stats = k.gn_fwd(x, gamma, beta, groups, act="none")
+    _check_stats(stats, x, groups, "%s %g" % (where, far))
+    ref, xh, _ = _ref(x, gamma, beta, groups, 1e-5, "none")
+    mean, rstd, mag = _ref_stats(x, groups, 1e-5)
+    mag = (mag * rstd).repeat_interleave(c // groups, -1).view(n, 1, 1, c)
+    _check(y, ref, gamma.double().abs() * (xh.abs() + mag) + beta.double().abs(), "y", chain=70)
+
+
+@pytest.mark.parametrize("shape,groups,two_passes", STAT_SHAPES)
+def test_gn_statistics_of_a_large_common_mean(shape, groups, two_passes):
+    """mean / std = 1e4 in f32, with and without a zero corner: the centres of a thread's values are of the mean's
+    size, and 2 U of that is 2e4 U of a standard deviation; what it moves the variance by is summed over at least
+    500 values with signs of their own: 2 * 2e4 U / sqrt(500) of it, half of that of rstd."""
+    k = _k()
+    g = torch.Generator(device="cuda").manual_seed(12)
+    x = torch.randn(shape, generator=g, device="cuda") + 1e4
+    ones = torch.ones(shape[-1], device="cuda")
+    for corner in (False, True):
+        if corner:
+            x[:, 0, 0, ::shape[-1] // groups] = 0
+        _, stats = k.gn_fwd(x, ones, ones, groups, act="none")
+        mean, rstd, _ = _ref_stats(x, groups, 1e-5)
+        m = x[0].numel() // groups
+        err = ((stats[..., 1].double() - rstd).abs() / rstd).max().item()
+        assert err <= 60 * U + 4 * 2e4 * U / m ** 0.5, "corner %s: rstd is %.3g off" % (corner, err)
+        assert ((stats[..., 0].double() - mean).abs() <= 4 * U * 1e4).all()
