@@ -74,6 +74,7 @@ _SIGS = {
     "dtp_gn_bwd": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float, c_float,
                    c_void_p, c_size_t, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
     "dtp_ns_workspace": [c_int, c_void_p, c_void_p],
+    "dtp_ns_tile": [c_int, c_int, c_int],
     "dtp_newton_schulz": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_float,
                           c_void_p, c_size_t, c_void_p],
     "dtp_muon_step": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float, c_int, c_float,

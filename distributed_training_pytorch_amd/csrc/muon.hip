@@ -1032,7 +1032,8 @@ template <int F, int EPI> int launch_tiles(const NsCall& c, const NsGemm& p, boo
 // in units of a 64 x 64 tile's, from chains of equal products: 2048 x 2048 (us in all) 128: 888, 64: 889, 32: 994, 192:
 // 1315; 4096 x 4096 192: 3659, 64: 4878, 128: 4996, 32: 7166; 1024 x 1024 64: 220, 32: 263, 128: 487; 512 x 512 32: 6.2
 // a product, 64: 8.3.
-template <int EPI> int gemm(const NsCall& c, const NsGemm& p) {
+// shared: whether K is cut between workgroups.
+template <int EPI> int tile_side(const NsCall& c, const NsGemm& p, bool& shared) {
   const int side[4] = {192, 128, 64, 32};
   const double cost[4] = {5.5, 3.0, 1.0, 0.4};
   long n[4];
@@ -1042,16 +1043,24 @@ template <int EPI> int gemm(const NsCall& c, const NsGemm& p) {
     for (int i = 0; i < c.count; ++i) n[v] += tiles<EPI>(c, p, i, side[v], side[v]);
     if ((double)((n[v] + 255) / 256) * cost[v] < (double)((n[best] + 255) / 256) * cost[best]) best = v;
   }
+  shared = false;
   if (EPI == EPI_PAIR && p.op[0].a == W_X && n[2] <= NS_SHARED) {
     // few tiles and a long K (the Gram matrix of 512 x 4608): 17 us shared out, adding up included; 28 otherwise
     int nk = 0;
     for (int i = 0; i < c.count; ++i) nk = nk < c.tb.mat[i].n / 32 ? c.tb.mat[i].n / 32 : nk;
-    if (nk >= 64) return launch_tiles<4, EPI_PAIR>(c, p, true);
+    shared = nk >= 64;
   }
-  if (best == 0) return launch_gemm<192, 192, 2, 4, 3, EPI>(c, p);
-  if (best == 1) return launch_gemm<128, 128, 2, 2, 4, EPI>(c, p);
-  if (best == 2) return launch_tiles<4, EPI>(c, p, false);
-  return launch_tiles<2, EPI>(c, p, false);
+  return shared ? 64 : side[best];
+}
+
+template <int EPI> int gemm(const NsCall& c, const NsGemm& p) {
+  bool shared;
+  const int side = tile_side<EPI>(c, p, shared);
+  if (side == 192) return launch_gemm<192, 192, 2, 4, 3, EPI>(c, p);
+  if (side == 128) return launch_gemm<128, 128, 2, 2, 4, EPI>(c, p);
+  if (side == 32) return launch_tiles<2, EPI>(c, p, false);
+  if (EPI == EPI_PAIR && shared) return launch_tiles<4, EPI_PAIR>(c, p, true);
+  return launch_tiles<4, EPI>(c, p, false);
 }
 
 template <int KIND, int MUON>
@@ -1222,6 +1231,22 @@ extern "C" size_t dtp_ns_workspace(int count, const int* rows, const int* cols) 
   NsCall c;
   if (fill_table(c, count, rows, cols)) return 0;
   return (size_t)ns_bytes(c);
+}
+
+// Tile side that a product of one matrix's chain is worked off in (by launches; matrices for one workgroup have none: 0).
+// product: 0 the Gram matrix, 1 the polynomial, 2 P A and P Q together, 3 Q X between segments, 4 the last Q X.
+extern "C" int dtp_ns_tile(int rows, int cols, int product) {
+  NsCall c;
+  if (fill_table(c, 1, &rows, &cols) || product < 0 || product > 4) return -10;
+  ns_layout(c);
+  if (ns_is_small(c)) return 0;
+  NsGemm p = {};
+  bool shared;
+  p.nops = product == 2 ? 2 : 1;
+  p.is_long = product >= 3;
+  p.op[0].a = product == 0 ? W_X : W_P;
+  return product == 1 ? tile_side<EPI_POLY>(c, p, shared) : product == 4 ? tile_side<EPI_OUT>(c, p, shared)
+                                                                          : tile_side<EPI_PAIR>(c, p, shared);
 }
 
 // out[i] = Newton-Schulz of src[i] ([rows][cols], contiguous).  in_kind / out_kind: 0 f32, 1 bf16, 2 f16.

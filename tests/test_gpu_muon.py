@@ -214,3 +214,57 @@ def test_muon_repeats_bit_for_bit_on_streams_and_in_graphs():
             for x, y in zip(st, w):
                 for t, u in zip(x, y):
                     assert torch.equal(t, u)
+
+
+def _tol_of_long_sums(m):
+    """NS_TOL plus what sums of m products lose.  Behind three steps Q is a^3 I and a matrix of about a^3 / m: Q X adds up
+    one term a^3 X and m small ones that cancel it, in m / 32 instructions, each of which rounds a partial sum (between
+    a^3 X and X, squares a third of the first's on average) off by up to 2^-23 of it (3^-1/2 of that on average; the unit
+    need not round to nearest).  The second segment multiplies what lies across G's directions by a^2: an error of
+    a^5 2^-23 / 3 = 1.9e-5 an instruction, independent of each other, next to the 1e-4 that NS_TOL is twice of.  (At
+    1980 x 2010 and rank one 2.0e-4, at 4150 x 4210 3.0e-4; a loop of f32 products 3.7e-4 and 5.2e-4, by the same sums.)"""
+    return 2 * math.sqrt((NS_TOL / 2) ** 2 + m / 32 * (COEFFS[0] ** 5 * 2.0 ** -23 / 3) ** 2)
+
+
+# m x n, and the tile sides of: Gram, polynomial, P A with P Q, Q X between segments, last Q X.  No side a multiple of 128
+# or 192.
+TILED = [(1980, 2010, (64, 64, 64, 128, 128)), (2450, 2530, (128, 128, 192, 192, 192)), (4150, 4210, (192, 192, 192, 192, 192))]
+
+
+@pytest.mark.parametrize("kind", ["full", "noise", "rank1"])
+@pytest.mark.parametrize("tall", [False, True])
+@pytest.mark.parametrize("m,n,sides", TILED)
+def test_newton_schulz_in_large_tiles(m, n, sides, tall, kind):
+    """The 192- and 128-wide tiles (staged through LDS) in every product of the chain, with tiles that end inside the
+    matrix."""
+    from distributed_training_pytorch_amd import _lib
+    rows, cols = (n, m) if tall else (m, n)
+    assert tuple(_lib.hip().dtp_ns_tile(rows, cols, p) for p in range(5)) == sides
+    g = _matrix(rows, cols, kind, seed=rows)
+    o = _k().newton_schulz(g, out_dtype=F32)
+    assert _rel(o, _ns64(g)) <= _tol_of_long_sums(m)
+    if kind == "noise":                                # a wrong tile is off by its own size, roundings spread over the rows
+        d = (o.double() - _ns64(g)).abs()
+        rows_off = (d.norm(dim=1) / _ns64(g).norm(dim=1)).max().item()
+        assert rows_off <= 10 * _tol_of_long_sums(m)
+        assert torch.equal(_k().newton_schulz(g.to(BF16).float(), out_dtype=F16), _k().newton_schulz(g.to(BF16), out_dtype=F16))
+
+
+def test_muon_step_of_large_matrices_beside_small_ones():
+    """Matrices with a short side above 1024 are worked off alone, the others together, in any order of the list."""
+    k = _k()
+    shapes = [(64, 576), (2450, 2530), (30, 70), (2530, 2450), (1100, 1200), (512, 300)]
+    ps, gs, ms = _muon_state(shapes, F32)
+    lps = [torch.zeros_like(p, dtype=BF16) for p in ps]
+    w64, m64 = [p.double() for p in ps], [m.double() for m in ms]
+    lr, mu, wd = 0.02, 0.95, 0.1
+    k.muon_step(ps, gs, ms, lps, lr=lr, momentum=mu, weight_decay=wd)
+    for i, s in enumerate(shapes):
+        d = gs[i].double()
+        m64[i] = mu * m64[i] + (1 - mu) * d
+        o = _ns64((1 - mu) * d + mu * m64[i])
+        adj = 0.2 * math.sqrt(max(s))
+        w64[i] = w64[i] * (1 - lr * wd) - lr * adj * o
+        assert (ms[i].double() - m64[i]).norm() <= 4 * 2.0 ** -24 * (m64[i].norm() + d.norm())
+        assert (ps[i].double() - w64[i]).norm() <= lr * adj * _tol_of_long_sums(min(s)) * o.norm() + 4 * 2.0 ** -24 * w64[i].norm(), s
+        assert torch.equal(lps[i], ps[i].to(BF16))
