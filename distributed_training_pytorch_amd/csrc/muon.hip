@@ -679,10 +679,14 @@ __host__ __device__ inline int segment_steps(int steps, int seg) {
   return steps / n + (seg < steps % n ? 1 : 0);
 }
 
+// scale / |G| as mantissa and power of two: the number itself leaves f32 for |G| below 2.4e-35 (a zero matrix times
+// infinity), and v * 2^e first is exact.
+struct NsFactor { float mant; int e; };
+
 // 8 values of X along memory or across it: elements i0, i0 + stride, ... of G, `have` of them (the rest zero)
 template <int KIND, int MUON>
-DTP_DEVINL void ns_load8(const NsMat& t, const MuonArgs& ma, const long i0, const int stride, const int have, const float inv,
-                         float* v) {
+DTP_DEVINL void ns_load8(const NsMat& t, const MuonArgs& ma, const long i0, const int stride, const int have,
+                         const NsFactor inv, float* v) {
   float m[8];
   if (stride == 1 && have == 8 && t.aligned && (i0 & 7) == 0) {
     if (KIND == 0) {
@@ -714,7 +718,7 @@ DTP_DEVINL void ns_load8(const NsMat& t, const MuonArgs& ma, const long i0, cons
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     if (MUON) v[e] = muon_again(v[e], m[e], ma);
-    v[e] *= inv;
+    v[e] = ldexpf(v[e], inv.e) * inv.mant;
   }
 }
 
@@ -805,7 +809,8 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsTable tb, char* _
   for (int seg = 0; seg < nseg; ++seg) {
     const int ns = segment_steps(q.steps, seg);
     const float sx = q.scale[sc];
-    const float inv0 = (float)((double)sx / norm);
+    NsFactor inv0;
+    inv0.mant = (float)frexp((double)sx / norm, &inv0.e);
     // 8 neighbouring values along n of row r of X, times its scale
     auto load_x = [&](int r, int k, float* v) {
       if (seg == 0) {

@@ -1217,8 +1217,8 @@ def _ns_check_schedule(steps, coeffs, eps):
         raise ValueError("newton_schulz: steps must be 1..%d, got %r" % (NS_MAX_STEPS, steps))
     if len(coeffs) != 3 or not all(_math.isfinite(v) for v in coeffs):
         raise ValueError("newton_schulz: coeffs must be three finite numbers, got %r" % (coeffs,))
-    if not (_math.isfinite(eps) and eps > 0):
-        raise ValueError("newton_schulz: eps must be positive, got %r" % (eps,))
+    if not 0.0 < _ctypes.c_float(eps).value < _math.inf:
+        raise ValueError("newton_schulz: eps must be positive in f32, got %r" % (eps,))
     return _ns_plan(int(steps), tuple(float(v) for v in coeffs))
 
 

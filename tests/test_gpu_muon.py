@@ -268,3 +268,18 @@ def test_muon_step_of_large_matrices_beside_small_ones():
         assert (ms[i].double() - m64[i]).norm() <= 4 * 2.0 ** -24 * (m64[i].norm() + d.norm())
         assert (ps[i].double() - w64[i]).norm() <= lr * adj * _tol_of_long_sums(min(s)) * o.norm() + 4 * 2.0 ** -24 * w64[i].norm(), s
         assert torch.equal(lps[i], ps[i].to(BF16))
+
+
+@pytest.mark.parametrize("rows,cols", [(64, 64), (7, 50), (100, 128), (900, 40), (200, 300)])
+@pytest.mark.parametrize("eps", [1e-37, 1e-40])
+def test_newton_schulz_of_zero_and_next_to_it(rows, cols, eps):
+    """1 / (|G| + eps) leaves f32 here; X_0 does not.  (eps is an f32 in the formula: 1e-40 is 7e-6 off as one.)"""
+    k = _k()
+    assert (k.newton_schulz(torch.zeros(rows, cols, device="cuda"), eps=eps, out_dtype=F32) == 0).all()
+    for size in (1e-38, 1e-36):
+        g = _matrix(rows, cols, "full") * size
+        assert _rel(k.newton_schulz(g, eps=eps, out_dtype=F32), _ns64(g, eps=torch.tensor(eps, dtype=F32).item())) <= NS_TOL
+    ps, gs, ms = [torch.randn(rows, cols, device="cuda")], [torch.zeros(rows, cols, device="cuda")], [torch.zeros(rows, cols, device="cuda")]
+    was = ps[0].clone()
+    k.muon_step(ps, gs, ms, [None], lr=0.5, weight_decay=0.0, eps=eps)
+    assert torch.equal(ps[0], was)

@@ -21,6 +21,9 @@ Z = torch.zeros
     (lambda: K.newton_schulz(Z(4, 4), coeffs=(1.0, 2.0, float("nan"))), "three"),
     (lambda: K.newton_schulz(Z(4, 4), coeffs=(30.0, 1.0, 1.0)), "bounded"),
     (lambda: K.newton_schulz(Z(4, 4), eps=0.0), "eps"),
+    (lambda: K.newton_schulz(Z(4, 4), eps=1e-50), "eps"),
+    (lambda: K.newton_schulz(Z(4, 4), eps=1e39), "eps"),
+    (lambda: K.newton_schulz(Z(4, 4), eps=float("nan")), "eps"),
     (lambda: K.newton_schulz(Z(4, 4), out_dtype=torch.float64), "out_dtype"),
     (lambda: K.newton_schulz(Z(1).expand(1, 2 ** 20 + 1).contiguous()), "2\\^20"),
     (lambda: K.newton_schulz(Z(4, 4)), "CUDA"),
