@@ -10,8 +10,10 @@
 // kernel sums in a fixed order (no atomics: results repeat bit for bit).
 //
 // Variance: every thread takes the mean c of a few values that it holds and M = sum of (x - c)^2 around it; sets of n values
-// meet as  M = sum of M_t + n_t (c_t - mean)^2,  in f64 between threads and pieces.  Nothing but squares is added, so neither
-// a mean far from zero nor a value far from the others cancels: rstd is good to a few units of f32 whatever the data.
+// meet as  M = sum of M_t + n_t (c_t - mean)^2.  Nothing but squares is added, so neither a mean far from zero nor a value
+// far from the others cancels: rstd is good to a few units of f32 whatever the data.  Between threads and pieces sets meet
+// in f64 and in one pass, around the first set's c: M = sum of M_t + n_t d_t^2 - (sum of n_t d_t)^2 / n with d_t = c_t - c_0.
+// What that cancels is n (c_0 - mean)^2 of at least n_0 (c_0 - mean)^2: n / n_0 units of f64's 2^-53.
 // (Sums around one value of the group, its first: 5e-5 off where that value lies 30 standard deviations from the mean,
 // 2e-3 at 300.  E[x^2] - mean^2 loses mean^2 / var * 6e-8.)
 #include "dtp_common.h"
@@ -122,6 +124,8 @@ DTP_DEVINL double wave_reduce_sum_f64(double v) {
   v += __shfl_xor(v, 16, 64);
   return v + __shfl_xor(v, 32, 64);
 }
+
+DTP_DEVINL double not_negative(double v) { return v < 0.0 ? 0.0 : v; }      // NaN stays NaN
 
 struct GnShape {
   int N, HW, C, G, cpg;      // cpg = C / G
@@ -284,20 +288,19 @@ __global__ __launch_bounds__(NT) void gn_slab_fwd_kernel(const void* __restrict_
   const int lane = threadIdx.x & 63;
   const double mm = (double)s.HW * s.cpg;
   for (int g = threadIdx.x >> 6; g < ng; g += NT / 64) {
+    const double first = (double)sm[g * m] + (double)sm[plane + g * m];
     double a = 0.0, v = 0.0;
     for (int i = lane; i < R * m; i += 64) {
       const int r = i / m, j = r * row + g * m + i - r * m;
-      a += (double)(dealt(r) * u) * ((double)sm[j] + (double)sm[plane + j]);
+      const double d = ((double)sm[j] + (double)sm[plane + j]) - first, nd = (double)(dealt(r) * u) * d;
+      a += nd;
+      v += fma(nd, d, (double)sm[2 * plane + j]);
     }
-    const double mean = wave_reduce_sum_f64(a) / mm;
-    for (int i = lane; i < R * m; i += 64) {
-      const int r = i / m, j = r * row + g * m + i - r * m;
-      const double d = ((double)sm[j] + (double)sm[plane + j]) - mean;
-      v += (double)sm[2 * plane + j] + (double)(dealt(r) * u) * d * d;
-    }
-    v = wave_reduce_sum_f64(v);
+    a = wave_reduce_sum_f64(a) / mm;
+    v = wave_reduce_sum_f64(v) / mm;
     if (lane == 0) {
-      const float rstd = (float)(1.0 / sqrt(v / mm + (double)eps));
+      const double mean = first + a;
+      const float rstd = (float)(1.0 / sqrt(not_negative(fma(-a, a, v)) + (double)eps));
       ms[2 * g] = (float)mean;
       ms[2 * g + 1] = rstd;
       float* o = stats + ((size_t)n * s.G + g0 + g) * 2;
@@ -608,20 +611,32 @@ __global__ __launch_bounds__(GN_T) void gn_partial_kernel(const void* __restrict
         }
       }
     } else {
-      for (int j = threadIdx.x; j < TX * VEC; j += GN_T) {
-        const int c = cb * VEC + j, len = r1 - r0;
-        if (c < s.C) {
-          const Deal dealt(len, R);
-          const auto mean_of = [&](int k) { return (double)thr[2 * GN_T * VEC + k * TX * VEC + j] + (double)thr[k * TX * VEC + j]; };
-          double a = 0.0, v = 0.0;
-          for (int k = 0; k < R; ++k) a += (double)dealt(k) * mean_of(k);
-          a /= (double)len;
-          for (int k = 0; k < R; ++k) {
-            const double d = mean_of(k) - a;
-            v += (double)thr[GN_T * VEC + k * TX * VEC + j] + (double)dealt(k) * d * d;
+      // P neighbouring lanes a channel, where channels are fewer than threads
+      int P = 1;
+      while (P < 64 && 2 * P * TX * VEC <= GN_T) P *= 2;
+      const int len = r1 - r0, q = threadIdx.x & (P - 1);
+      const Deal dealt(len, R);
+      for (int j = threadIdx.x / P; j - (int)threadIdx.x / P < TX * VEC; j += GN_T / P) {
+        const int c = cb * VEC + j;
+        const auto mean_of = [&](int k) { return (double)thr[2 * GN_T * VEC + k * TX * VEC + j] + (double)thr[k * TX * VEC + j]; };
+        const bool mine = j < TX * VEC && c < s.C;
+        const double first = mine ? mean_of(0) : 0.0;
+        double a = 0.0, v = 0.0;
+        if (mine) {
+#pragma unroll 4
+          for (int k = q; k < R; k += P) {
+            const double d = mean_of(k) - first, nd = (double)dealt(k) * d;
+            a += nd;
+            v += fma(nd, d, (double)thr[GN_T * VEC + k * TX * VEC + j]);
           }
-          chm[c] = a;
-          chv[c] = (float)v;
+        }
+        for (int off = 1; off < P; off *= 2) {
+          a += __shfl_xor(a, off, 64);
+          v += __shfl_xor(v, off, 64);
+        }
+        if (mine && q == 0) {
+          chm[c] = first + a / (double)len;
+          chv[c] = (float)not_negative(v - a * a / (double)len);
         }
       }
     }
@@ -630,15 +645,18 @@ __global__ __launch_bounds__(GN_T) void gn_partial_kernel(const void* __restrict
   if (!BWD) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     for (int g = wave; g < s.G; g += GN_T / 64) {
+      const double first = chm[g * s.cpg], len = (double)(r1 - r0);
       double a = 0.0, v = 0.0;
-      for (int c = lane; c < s.cpg; c += 64) a += chm[g * s.cpg + c];
-      a = wave_reduce_sum_f64(a) / (double)s.cpg;
       for (int c = lane; c < s.cpg; c += 64) {
-        const double d = chm[g * s.cpg + c] - a;
-        v += (double)chv[g * s.cpg + c] + (double)(r1 - r0) * d * d;
+        const double d = chm[g * s.cpg + c] - first;
+        a += d;
+        v += fma(len * d, d, (double)chv[g * s.cpg + c]);
       }
+      a = wave_reduce_sum_f64(a);
       v = wave_reduce_sum_f64(v);
       if (lane == 0) {
+        v = not_negative(v - len * a * a / (double)s.cpg);
+        a = first + a / (double)s.cpg;
         float* o = partial + (((size_t)n * s.chunks + chunk) * s.G + g) * 3;
         o[0] = (float)a;
         o[1] = (float)(a - (double)(float)a);
@@ -656,21 +674,20 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const float* __restrict__
   if (idx >= (long)s.N * s.G) return;
   const int n = (int)(idx / s.G), g = (int)(idx - (long)n * s.G);
   const float* pn = partial + ((size_t)n * s.chunks * s.G + g) * 3;
+  const double first = (double)pn[0] + (double)pn[1];
   double a = 0.0, v = 0.0;
+#pragma unroll 4
   for (int k = lane; k < s.chunks; k += 64) {
     const float* o = pn + (size_t)k * s.G * 3;
-    a += (double)min(s.rows, s.HW - k * s.rows) * ((double)o[0] + (double)o[1]);
+    const double d = ((double)o[0] + (double)o[1]) - first, nd = (double)min(s.rows, s.HW - k * s.rows) * d;
+    a += nd;
+    v += fma(nd * (double)s.cpg, d, (double)o[2]);
   }
   a = wave_reduce_sum_f64(a) / (double)s.HW;
-  for (int k = lane; k < s.chunks; k += 64) {
-    const float* o = pn + (size_t)k * s.G * 3;
-    const double d = ((double)o[0] + (double)o[1]) - a;
-    v += (double)o[2] + (double)min(s.rows, s.HW - k * s.rows) * (double)s.cpg * d * d;
-  }
-  v = wave_reduce_sum_f64(v);
+  v = wave_reduce_sum_f64(v) / ((double)s.HW * s.cpg);
   if (lane == 0) {
-    stats[idx * 2] = (float)a;
-    stats[idx * 2 + 1] = (float)(1.0 / sqrt(v / ((double)s.HW * s.cpg) + (double)eps));
+    stats[idx * 2] = (float)(first + a);
+    stats[idx * 2 + 1] = (float)(1.0 / sqrt(not_negative(fma(-a, a, v)) + (double)eps));
   }
 }
 
