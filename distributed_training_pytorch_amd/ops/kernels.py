@@ -1003,6 +1003,17 @@ def _gn_check(x, groups, act, *vecs):
     return dims
 
 
+def _gn_check_writes(dgamma, dbeta, *read):
+    """The parameter gradients are written while other workgroups still read: their bytes are nobody else's."""
+    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (dgamma, dbeta) + read]
+    for i in (0, 1):
+        lo, hi = spans[i]
+        for a, b in spans[i + 1:]:
+            if a < hi and lo < b:
+                raise ValueError("gn_bwd: dgamma and dbeta share their memory with each other or with what is read (x, dy, "
+                                 "gamma, beta, stats)")
+
+
 @_functools.lru_cache(maxsize=256)
 def _gn_workspace(N, HW, C, G, dt, bwd):
     n = _lib.hip().dtp_gn_workspace(N, HW, C, G, dt, bwd)
@@ -1046,8 +1057,7 @@ def gn_bwd(x, dy, gamma, beta, stats, groups, dgamma, dbeta, act="relu", beta_g=
             or dbeta.numel() != C or not dgamma.is_contiguous() or not dbeta.is_contiguous() \
             or dgamma.device != x.device or dbeta.device != x.device:
         raise ValueError("gn_bwd: dgamma / dbeta must be contiguous [C] of one dtype (f32 / bf16) on x's device")
-    if len({dgamma.data_ptr(), dbeta.data_ptr()} - {gamma.data_ptr(), beta.data_ptr()}) < 2:
-        raise ValueError("gn_bwd: dgamma and dbeta share their memory with each other or with gamma / beta")
+    _gn_check_writes(dgamma, dbeta, x, dy, gamma, beta, stats)
     dx = torch.empty_like(x)
     if N == 0:
         if beta_g == 0.0:

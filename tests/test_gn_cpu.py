@@ -40,3 +40,29 @@ def test_more_threads_than_a_launch_holds(bwd):
         K._gn_workspace(1 << 24, 1, 32, 4, 0, bwd)
     with pytest.raises(ValueError, match="refuses"):
         K._gn_workspace(1 << 22, 1, 4096, 4096, 0, bwd)
+
+
+@pytest.mark.parametrize("which", ["each other, in part", "each other, bf16", "in x", "in dy", "gamma, in part", "beta, in part", "in stats"])
+def test_gn_parameter_gradients_share_no_memory(which):
+    c = 16
+    x, dy, stats = torch.zeros(2, 3, c), torch.zeros(2, 3, c), torch.zeros(2, 4, 2)
+    gamma, beta, dg, db, flat = torch.ones(c), torch.zeros(c), torch.zeros(c), torch.zeros(c), torch.zeros(3 * c)
+    K._gn_check_writes(dg, db, x, dy, gamma, beta, stats)
+    K._gn_check_writes(flat[:c], flat[c:2 * c], x, dy, flat[2 * c:], beta, stats)       # side by side
+    if which == "each other, in part":
+        dg, db = flat[:c], flat[c - 1:2 * c - 1]
+    elif which == "each other, bf16":
+        dg, db = flat.bfloat16()[:c], None
+        db = dg[c - 1:]
+    elif which == "in x":
+        dg = x.view(-1)[c:2 * c]
+    elif which == "in dy":
+        db = dy.view(-1)[2 * c:3 * c]
+    elif which == "gamma, in part":
+        gamma, dg = flat[:c], flat[c // 2:c // 2 + c]
+    elif which == "beta, in part":
+        beta, dg = flat[4:4 + c], flat[:c]
+    else:
+        db = stats.view(-1)[:c]
+    with pytest.raises(ValueError, match="share their memory"):
+        K._gn_check_writes(dg, db, x, dy, gamma, beta, stats)

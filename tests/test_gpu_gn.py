@@ -346,3 +346,13 @@ def test_gn_statistics_of_a_large_common_mean(shape, groups, two_passes):
         err = ((stats[..., 1].double() - rstd).abs() / rstd).max().item()
         assert err <= 60 * U + 4 * 2e4 * U / m ** 0.5, "corner %s: rstd is %.3g off" % (corner, err)
         assert ((stats[..., 0].double() - mean).abs() <= 4 * U * 1e4).all()
+
+
+def test_gn_bwd_refuses_parameter_gradients_inside_what_is_read():
+    k = _k()
+    x, dy, gamma, beta = _inputs((2, 3, 3, 16), F32)
+    _, stats = k.gn_fwd(x, gamma, beta, 4)
+    d, flat = torch.zeros(16, device="cuda"), torch.zeros(40, device="cuda")
+    for dg, db in ((x.view(-1)[:16], d), (d, dy.view(-1)[16:32]), (stats.view(-1), d), (flat[:16], flat[12:28])):
+        with pytest.raises(ValueError, match="share their memory"):
+            k.gn_bwd(x, dy, gamma, beta, stats, 4, dg, db)
