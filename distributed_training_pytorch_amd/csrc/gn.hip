@@ -862,9 +862,10 @@ GnShape shape_of(int N, int HW, int C, int G, int vec, int elem, int bwd) {
   return s;
 }
 
+// (HW: kernels count rows in 32 bits, up to a piece's 2^20 rows past the end before they compare)
 bool gn_ok(int N, int HW, int C, int G, int dtype, int act) {
   return N > 0 && HW > 0 && C > 0 && C <= GN_MAXC && G > 0 && C % G == 0 && dtype >= 0 && dtype <= 2 && act >= 0 &&
-         act <= 2 && (long)HW * C < 0x7fffffffL && (long)N * HW < 0x7fffffffL;
+         act <= 2 && (long)HW < 0x80000000L - (1L << 21) && (long)HW * C < 0x7fffffffL && (long)N * HW < 0x7fffffffL;
 }
 
 // widest vector of at most 16 bytes that divides a row

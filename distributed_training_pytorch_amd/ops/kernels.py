@@ -984,8 +984,9 @@ def _gn_shape(shape, groups):
         HW *= d
     if HW == 0 and N > 0:
         raise ValueError("group norm: no values to normalise in %s" % (tuple(shape),))
-    if HW * C >= 2 ** 31 - 1 or N * HW >= 2 ** 31 - 1:
-        raise ValueError("group norm: %s is too large (2^31 values an image, 2^31 pixels)" % (tuple(shape),))
+    if HW * C >= 2 ** 31 - 1 or N * HW >= 2 ** 31 - 1 or HW >= 2 ** 31 - 2 ** 21:
+        raise ValueError("group norm: %s is too large (2^31 values an image, 2^31 pixels, 2^31 - 2^21 pixels an image)" %
+                         (tuple(shape),))
     return N, HW, C, G
 
 

@@ -19,6 +19,7 @@ def _fwd(x, groups=4, act="relu", gamma=None, beta=None):
     (lambda: _fwd(torch.zeros(1, 1, 4100)), "at most 4096"),
     (lambda: _fwd(torch.zeros(2, 0, 16)), "no values"),
     (lambda: _fwd(torch.zeros(1, dtype=torch.bfloat16).expand(1, 2 ** 27, 16)), "too large"),
+    (lambda: _fwd(torch.zeros(1, dtype=torch.bfloat16).expand(1, 2 ** 31 - 2 ** 21, 1), groups=1), "too large"),
     (lambda: _fwd(torch.zeros(2, 3, 16), gamma=torch.ones(15)), "gamma / beta"),
     (lambda: _fwd(torch.zeros(2, 3, 16), beta=torch.ones(16, dtype=torch.bfloat16)), "gamma / beta"),
     (lambda: _fwd(torch.zeros(2, 3, 16)), "must be a CUDA tensor"),
@@ -66,3 +67,12 @@ def test_gn_parameter_gradients_share_no_memory(which):
         db = stats.view(-1)[:c]
     with pytest.raises(ValueError, match="share their memory"):
         K._gn_check_writes(dg, db, x, dy, gamma, beta, stats)
+
+
+@pytest.mark.parametrize("bwd", [0, 1])
+def test_rows_whose_count_would_pass_32_bits(bwd):
+    """One channel and nearly 2^31 pixels: a piece's end, or a thread's next row behind it, is a negative number."""
+    assert K._gn_workspace(1, 2 ** 31 - 2 ** 21 - 1, 1, 1, 0, bwd) > 0
+    for hw in (2 ** 31 - 2 ** 21, 2 ** 31 - 2):
+        with pytest.raises(ValueError, match="refuses"):
+            K._gn_workspace(1, hw, 1, 1, 0, bwd)

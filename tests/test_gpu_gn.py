@@ -356,3 +356,32 @@ def test_gn_bwd_refuses_parameter_gradients_inside_what_is_read():
     for dg, db in ((x.view(-1)[:16], d), (d, dy.view(-1)[16:32]), (stats.view(-1), d), (flat[:16], flat[12:28])):
         with pytest.raises(ValueError, match="share their memory"):
             k.gn_bwd(x, dy, gamma, beta, stats, 4, dg, db)
+
+
+def test_gn_of_one_channel_and_two_thousand_million_pixels():
+    """The longest image that is taken: row numbers up to 2^31 - 2^21.  (Sums of a thread: 4,100 rows.)"""
+    k = _k()
+    hw = 2 ** 31 - 2 ** 21 - 1
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.empty((1, hw, 1), device="cuda", dtype=BF16)
+    part = 1 << 28
+    for i in range(0, hw, part):
+        v = x[0, i:i + part, 0]
+        v.copy_(torch.randn(v.shape, generator=g, device="cuda") + i / hw)
+    one, zero = torch.ones(1, device="cuda"), torch.zeros(1, device="cuda")
+    y, stats = k.gn_fwd(x, one, zero, 1, act="none")
+    pieces = [x[0, i:i + part, 0] for i in range(0, hw, part)]
+    mean = sum(v.double().sum().item() for v in pieces) / hw
+    var = sum((v.double() - mean).square().sum().item() for v in pieces) / hw
+    rstd = (var + 1e-5) ** -0.5
+    # (runs of eight in a thread: 512 additions of squares, each U of the sum)
+    assert abs(stats[0, 0, 1].item() - rstd) <= 600 * U * rstd and abs(stats[0, 0, 0].item() - mean) <= 10 * U * (1 + mean)
+    for lo in (0, hw // 2, hw - 100_000):
+        _check(y[0, lo:lo + 100_000, 0], (x[0, lo:lo + 100_000, 0].double() - mean) * rstd, 1 + 0 * y[0, lo:lo + 100_000, 0].double(),
+               "y", chain=1200)
+    dg, db = torch.empty(1, device="cuda"), torch.empty(1, device="cuda")
+    dx = k.gn_bwd(x, y, one, zero, stats, 1, dg, db, act="none")
+    # dy = xhat: dgamma = sum xhat^2, dbeta = sum xhat, dx = 0 up to the rounding of y (2^-8 of it)
+    sq = sum((y[0, i:i + part, 0].double() * (x[0, i:i + part, 0].double() - mean) * rstd).sum().item() for i in range(0, hw, part))
+    assert abs(dg.item() - sq) <= 4200 * U * sq
+    assert dx[0, -100_000:].abs().max().item() <= 8 * 2.0 ** -8 * rstd and dx[0, :100_000].abs().max().item() <= 8 * 2.0 ** -8 * rstd
