@@ -6,6 +6,7 @@ launches on the caller's current HIP stream.  Tensors are internal-layout: activ
 ``[N, H, W, C]``, conv weights ``[Cout, 9*Cin]`` (tap-major, channel-minor), linear weights
 ``[out, in]``.
 """
+import collections as _collections
 import contextlib as _contextlib
 import ctypes as _ctypes
 import functools as _functools
@@ -1153,29 +1154,60 @@ def adamw_flat(p, g, m, v, lp, lr, beta1, beta2, eps, wd, grad_scale, step):
     check(rc, "adamw_flat")
 
 
+class AdamWRanges(_collections.namedtuple("AdamWRanges", "rows arena_end v_end")):
+    """Work table of :func:`adamw_ranges`: int64 [workgroups, 3] on the device, and where its last ranges end."""
+
+
 def adamw_range_table(spans, device):
-    """Work table of :func:`adamw_ranges`: ``spans`` = (first element in the arena, elements, first element in the
-    second moment's buffer), multiples of 4; cut into at most 1024 elements each."""
+    """Table for :func:`adamw_ranges`: ``spans`` = (first element in the arena, elements, first element in the second
+    moment's buffer), multiples of 4, none over another; cut into at most 1024 elements each."""
     rows = []
     for first, n, at in spans:
-        if first % 4 or n % 4 or at % 4 or n <= 0:
+        if first % 4 or n % 4 or at % 4 or n <= 0 or first < 0 or at < 0:
             raise ValueError("adamw_range_table: spans must be positive multiples of 4, got %s" % ((first, n, at),))
         for k in range(0, n, 1024):
             rows.append((first + k, min(1024, n - k), at + k))
-    return torch.tensor(rows, dtype=torch.int64).to(device)
+    if not rows:
+        raise ValueError("adamw_range_table: no spans")
+    for col in (0, 2):
+        ends = sorted((r[col], r[col] + r[1]) for r in rows)
+        if any(a[1] > b[0] for a, b in zip(ends, ends[1:])):
+            raise ValueError("adamw_range_table: spans that share elements")
+    return AdamWRanges(torch.tensor(rows, dtype=torch.int64).to(device), max(r[0] + r[1] for r in rows),
+                       max(r[2] + r[1] for r in rows))
 
 
 def adamw_ranges(p, g, m, v, lp, table, step, lr, beta1, beta2, eps, wd, grad_scale):
-    """AdamW on the ranges of ``table`` (:func:`adamw_range_table`); ``step``: device int32 [1], the number of this
-    step (1 for the first)."""
-    if step.dtype != torch.int32 or step.numel() != 1 or table.dtype != torch.int64 or table.shape[1] != 3 \
-            or not table.is_contiguous() or not step.is_cuda or not table.is_cuda:
-        raise ValueError("adamw_ranges: step must be a device int32, table adamw_range_table's")
+    """AdamW on the ranges of ``table`` (:func:`adamw_range_table`) of the arena: p, m f32, g f32 or bf16, lp bf16 or None,
+    of one length; v f32, the second moments' own buffer.  ``step``: device int32 [1], the number of this step (1 for the
+    first)."""
+    if not isinstance(table, AdamWRanges):
+        raise ValueError("adamw_ranges: table must be adamw_range_table's")
+    if g.dtype not in (torch.float32, BF16):
+        raise ValueError("adamw_ranges: g must be f32 or bf16, got %s" % (g.dtype,))
+    if step.dtype != torch.int32 or step.numel() != 1:
+        raise ValueError("adamw_ranges: step must be one int32")
     if not (0.0 < beta1 < 1.0 and 0.0 < beta2 < 1.0):
         raise ValueError("adamw_ranges: betas must be in (0, 1), got %r, %r" % (beta1, beta2))
+    rows = table.rows
+    for t in (g, m) + ((lp,) if lp is not None else ()):
+        if t.numel() != p.numel():
+            raise ValueError("adamw_ranges: p, g, m and lp must be of one length")
+    if table.arena_end > p.numel() or table.v_end > v.numel():
+        raise ValueError("adamw_ranges: the table reaches %d elements of the arena and %d of v, they have %d and %d" %
+                         (table.arena_end, table.v_end, p.numel(), v.numel()))
+    for t in (g, m, v, rows, step) + ((lp,) if lp is not None else ()):
+        if t.device != p.device:
+            raise ValueError("adamw_ranges: tensors on different devices")
+    _need(p, torch.float32, "p")
+    _need(g, g.dtype, "g")
+    _need(m, torch.float32, "m")
+    _need(v, torch.float32, "v")
+    if lp is not None:
+        _need(lp, BF16, "lp")
     with _on_device_of(p):
-        check(_lib.hip().dtp_adamw_ranges(ptr(p), ptr(g), int(g.dtype == BF16), ptr(m), ptr(v), ptr(lp), ptr(table),
-                                          table.shape[0], ptr(step), float(lr), float(beta1), float(beta2), _math.log(beta1),
+        check(_lib.hip().dtp_adamw_ranges(ptr(p), ptr(g), int(g.dtype == BF16), ptr(m), ptr(v), ptr(lp), ptr(rows),
+                                          rows.shape[0], ptr(step), float(lr), float(beta1), float(beta2), _math.log(beta1),
                                           _math.log(beta2), float(eps), float(wd), float(grad_scale), stream()),
               "adamw_ranges")
 

@@ -98,3 +98,31 @@ def test_scales_keep_every_matrix_of_the_chain_in_f16(steps, coeffs):
             for v, s in ((lam, sa), (r, sa), (p, sp), (q, sq)):
                 assert v.abs().max() * s <= 16384
     assert not sc
+
+
+def _adamw(p=Z(64), g=Z(64), m=Z(64), v=Z(32), lp=Z(64, dtype=BF16), spans=((0, 16, 0), (32, 16, 16)), step=None):
+    step = torch.ones(1, dtype=torch.int32) if step is None else step
+    K.adamw_ranges(p, g, m, v, lp, K.adamw_range_table(spans, "cpu"), step, 1e-3, 0.9, 0.95, 1e-8, 0.1, 1.0)
+
+
+@pytest.mark.parametrize("call,what", [
+    (lambda: _adamw(g=Z(64, dtype=torch.float16)), "f32 or bf16"),           # 16-bit values read as 32-bit ones
+    (lambda: _adamw(g=Z(63)), "one length"),
+    (lambda: _adamw(m=Z(32)), "one length"),
+    (lambda: _adamw(lp=Z(32, dtype=BF16)), "one length"),
+    (lambda: _adamw(v=Z(28)), "reaches"),
+    (lambda: _adamw(spans=((0, 16, 0), (52, 16, 16))), "reaches"),
+    (lambda: _adamw(spans=((0, 16, 0), (12, 16, 16))), "share elements"),
+    (lambda: _adamw(spans=((0, 16, 0), (32, 16, 12))), "share elements"),
+    (lambda: _adamw(spans=((-4, 16, 0),)), "multiples of 4"),
+    (lambda: _adamw(spans=((0, 6, 0),)), "multiples of 4"),
+    (lambda: _adamw(spans=()), "no spans"),
+    (lambda: _adamw(step=torch.ones(1)), "int32"),
+    (lambda: K.adamw_ranges(Z(64), Z(64), Z(64), Z(64), None, torch.zeros(1, 3, dtype=torch.int64),
+                            torch.ones(1, dtype=torch.int32), 1e-3, 0.9, 0.95, 1e-8, 0.1, 1.0), "adamw_range_table's"),
+    (lambda: _adamw(), "CUDA tensor"),
+    (lambda: _adamw(lp=None), "CUDA tensor"),
+])
+def test_adamw_ranges_refusals(call, what):
+    with pytest.raises(ValueError, match=what):
+        call()
