@@ -32,6 +32,10 @@ def _synthetic_len(path, default):
     return None
 
 
+# (lr, momentum) where the caller names none: the reference's SGD; Muon's update is as large as AdamW's, and so is its lr
+OPTIMIZERS = {"sgd": (0.1, 0.9), "muon": (1e-3, 0.95)}
+
+
 class ExampleTrainer(Trainer):
     def __init__(self,
                  train_path,
@@ -48,8 +52,8 @@ class ExampleTrainer(Trainer):
                  save_folder='.',
                  snapshot_path=None,
                  logger=None,
-                 lr=0.1,
-                 momentum=0.9,
+                 lr=None,             # None: the optimizer's own, see OPTIMIZERS
+                 momentum=None,
                  weight_decay=1e-4,
                  milestones=(50, 100, 200),
                  batch_norm=False,
@@ -65,13 +69,16 @@ class ExampleTrainer(Trainer):
         self.labels = labels
         self.height = height
         self.width = width
-        self.lr, self.momentum, self.weight_decay = lr, momentum, weight_decay
         self.milestones = list(milestones)
         self.batch_norm = batch_norm
         self.group_norm = int(group_norm)            # groups of VGG16-GN's normalisation layers; 0: none
-        if optimizer not in ("sgd", "muon"):
-            raise ValueError("optimizer must be 'sgd' or 'muon', got %r" % (optimizer,))
+        if optimizer not in OPTIMIZERS:
+            raise ValueError("optimizer must be one of %s, got %r" % (sorted(OPTIMIZERS), optimizer))
         self.optimizer_name = optimizer
+        own_lr, own_momentum = OPTIMIZERS[optimizer]
+        self.lr = own_lr if lr is None else lr
+        self.momentum = own_momentum if momentum is None else momentum
+        self.weight_decay = weight_decay
         self.grad_dtype = grad_dtype
         self.fp8_classifier = fp8_classifier
         # ship uint8 pixels host->device and normalise inside the conv1 ingest kernel
@@ -128,7 +135,7 @@ class ExampleTrainer(Trainer):
 
     def build_optimizer(self):
         if self.optimizer_name == "muon":
-            return FusedMuon(self.model, lr=self.lr, weight_decay=self.weight_decay)
+            return FusedMuon(self.model, lr=self.lr, momentum=self.momentum, weight_decay=self.weight_decay)
         return FusedSGD(self.model, lr=self.lr, momentum=self.momentum, weight_decay=self.weight_decay)
 
     def build_scheduler(self):

@@ -27,7 +27,7 @@ def parse_args(argv=None):
     ap.add_argument("--image-size", type=int, default=224)
     ap.add_argument("--epochs", type=int, default=300)
     ap.add_argument("--batch-size", type=int, default=16, help="GLOBAL batch (split over ranks)")
-    ap.add_argument("--lr", type=float, default=0.1)
+    ap.add_argument("--lr", type=float, default=None, help="default: 0.1 for sgd, 0.001 for muon")
     ap.add_argument("--save-period", type=int, default=5)
     ap.add_argument("--save-folder", default="./runs")
     ap.add_argument("--snapshot", default=None, help="resume from this snapshot (e.g. runs/weights/last.pth)")
@@ -37,7 +37,7 @@ def parse_args(argv=None):
                     help="VGG16-GN variant: GroupNorm with this many groups behind every convolution (32 is usual)")
     ap.add_argument("--optimizer", default="sgd", choices=["sgd", "muon"],
                     help="sgd: momentum 0.9 (the reference's); muon: orthogonalised momentum for the weight matrices, AdamW "
-                         "for the rest (use an lr around 1e-3)")
+                         "for the rest")
     ap.add_argument("--uint8-input", action="store_true",
                     help="ship uint8 pixels to the GPU; /255, mean and std are fused into the conv1 ingest kernel")
     ap.add_argument("--fp8-classifier", action="store_true", help="linear1/linear2 forward GEMMs in OCP e4m3 (GPU)")

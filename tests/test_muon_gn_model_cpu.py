@@ -152,3 +152,19 @@ def test_main_runs_with_group_norm_and_muon(tmp_path):
     env = dict(os.environ, CUDA_VISIBLE_DEVICES="", HIP_VISIBLE_DEVICES="")
     r = subprocess.run(cmd, cwd=ROOT, env=env, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=600)
     assert r.returncode == 0, r.stdout[-3000:]
+
+
+@pytest.mark.parametrize("given,want", [
+    (dict(), (0.1, 0.9)), (dict(lr=0.02, momentum=0.5), (0.02, 0.5)), (dict(optimizer="muon"), (1e-3, 0.95)),
+    (dict(optimizer="muon", lr=0.02), (0.02, 0.95)), (dict(optimizer="muon", momentum=0.8), (1e-3, 0.8))])
+def test_trainer_gives_each_optimizer_its_own_lr_and_momentum(given, want, monkeypatch):
+    """Muon at SGD's lr of 0.1 moves every matrix by a tenth of its size a step; a momentum that is given counts."""
+    import main
+    from distributed_training_pytorch_amd.trainer.example_trainer import ExampleTrainer
+    from distributed_training_pytorch_amd.trainer.trainer import Trainer
+    monkeypatch.setattr(Trainer, "__init__", lambda self, *a, **k: None)
+    t = ExampleTrainer("train", "val", ["a"], 32, 32, 1, 2, False, **given)
+    t.model = Tiny()
+    g = t.build_optimizer().param_groups[0]
+    assert (g["lr"], g["momentum"]) == want
+    assert main.parse_args([]).lr is None
