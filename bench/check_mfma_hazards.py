@@ -9,7 +9,8 @@ assembly along fall-through AND branch targets and reports every such place.
 
   python bench/check_mfma_hazards.py [file.hip ...]      (default: every csrc/*.hip; exit 1 on a finding)
 
-It also fails on any kernel that needs scratch memory (``.amdhsa_private_segment_fixed_size`` > 0).
+It also fails on any kernel that needs scratch memory (``.amdhsa_private_segment_fixed_size`` > 0) and on packed f32
+arithmetic (``v_pk_add / mul / fma_f32``), which the build's flags are there to keep out.
 
 Wait states are counted the way LLVM's hazard recognizer does (one per instruction, ``s_nop N`` =
 N + 1), so an intervening independent MFMA counts 1 although it occupies the pipe for its passes —
@@ -29,7 +30,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "distributed_training_pytorch_amd", "csrc")
 HIPCC = "/opt/rocm/bin/hipcc"
 sys.path.insert(0, ROOT)
-from distributed_training_pytorch_amd._build import device_flags   # noqa: E402  (the flags the library is built with)
+from distributed_training_pytorch_amd._build import DEVICE_FLAGS   # noqa: E402  (the flags the library is built with)
 
 REG = re.compile(r"\bv\[(\d+):(\d+)\]|\bv(\d+)\b")
 LABEL = re.compile(r"^([.\w$]+):")
@@ -122,6 +123,10 @@ def check_kernel(name, ins, labels):
     return findings
 
 
+def packed_f32(ins):
+    return sum(1 for mn, _ in ins if re.match(r"v_pk_(add|mul|fma)_f32", mn))
+
+
 def main():
     files = sys.argv[1:] or sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
     bad = 0
@@ -131,7 +136,7 @@ def main():
         def to_asm(f):
             out = os.path.join(td, os.path.basename(f) + ".s")
             return out, subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=fast",
-                                        *device_flags(f), *defs, "-I", CSRC, "-S", "--cuda-device-only", "-o", out, f], capture_output=True, text=True)
+                                        *DEVICE_FLAGS, *defs, "-I", CSRC, "-S", "--cuda-device-only", "-o", out, f], capture_output=True, text=True)
         # the compilations are independent: run them side by side (igemm.hip alone takes a minute)
         import concurrent.futures
         with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(files), os.cpu_count() or 1)) as ex:
@@ -140,10 +145,14 @@ def main():
             if r.returncode != 0:
                 print("%s: does not compile to assembly\n%s" % (f, r.stderr[-2000:]))
                 return 2
-            n_mfma, found = 0, []
+            n_mfma, n_packed, found = 0, 0, []
             for name, (ins, labels) in parse(out).items():
                 n_mfma += sum(1 for mn, _ in ins if mn.startswith("v_mfma"))
                 found += check_kernel(name, ins, labels)
+                n_packed += packed_f32(ins)
+            if n_packed:
+                print("   %s: %d packed f32 instructions" % (os.path.basename(f), n_packed))
+            bad += n_packed
             # second check on the same assembly: no kernel of the tree may need scratch memory (a register
             # spill in an epilogue lambda once cost a 256x256 tile more than the feature it came with saved)
             txt = open(out).read()

@@ -24,14 +24,8 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
 # no packed f32 instructions (v_pk_add / mul / fma_f32): hipcc forms them from ordinary float code at -O3, and some
 # of their forms have given wrong results on this hardware now and then.  (The host pass warns that it does not
-# know the feature: harmless.)  igemm.hip keeps them: without them ten of its 32 kernels spill 24-132 bytes a lane,
-# and scratch traffic would enter the vmcnt counts that its pipelines wait on by hand.
-NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-PACKED_F32_SOURCES = ("igemm.hip",)
-
-
-def device_flags(src):
-    return [] if os.path.basename(src) in PACKED_F32_SOURCES else NO_PACKED_F32
+# know the feature: harmless.)
+DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _run(cmd):
@@ -55,7 +49,7 @@ def _compile_hip(src, headers, extra=()):
         # stamps of conv_c64, bench/stamp_c64.py); touch the source to force its rebuild
         defs = os.environ.get("DTP_BUILD_DEFS", "").split()
         _run([HIPCC, "--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast",
-              *device_flags(src), "-I", CSRC, *extra, *defs, "-c", src, "-o", obj])
+              *DEVICE_FLAGS, "-I", CSRC, *extra, *defs, "-c", src, "-o", obj])
     return obj
 
 

@@ -948,34 +948,31 @@ __global__ __launch_bounds__(WGM * WGN * 64) void igemm_nt_kernel(const IgemmPar
       }
     } else {
       // Fast path (every convolution): 128 accumulator values per lane at one wave-instruction per
-      // 4 cycles made this phase VALU-bound (4.5 us of a 256x256 tile).  Vector adds (v_pk_add_f32),
-      // one v_cvt_pk_bf16_f32 per pair, and ReLU AFTER the rounding as a packed signed-16-bit max
-      // on the bf16 bit patterns (negative floats are negative int16s; round(relu(x)) ==
-      // relu(round(x))), with the ReLU switch hoisted out of the loops.
-      auto body = [&](auto relu_tag) {
-        constexpr bool RELU = decltype(relu_tag)::value;
-        typedef short s16x2_t __attribute__((ext_vector_type(2)));
+      // 4 cycles made this phase VALU-bound (4.5 us of a 256x256 tile).  One v_cvt_pk_bf16_f32 per
+      // pair, and ReLU AFTER the rounding as a packed signed-16-bit max on the bf16 bit patterns
+      // (negative floats are negative int16s; round(relu(x)) == relu(round(x))): with 0, or without
+      // ReLU with the lowest int16, which changes nothing.  The bias goes through an empty asm: else
+      // hipcc adds it in front of the branches (dropout above adds it too) and spills 24-204 bytes.
+      typedef short s16x2_t __attribute__((ext_vector_type(2)));
+      const short lowest = p.relu ? 0 : -32768;
 #pragma unroll
-        for (int j = 0; j < NI; ++j) {
-          const int nl = wn * WN + j * 16 + cq;
-          const int q = nl >> 3, sub = ((nl >> 2) & 1) * 8;
+      for (int j = 0; j < NI; ++j) {
+        const int nl = wn * WN + j * 16 + cq;
+        f32x4_t b = bvv[j];
+        asm volatile("" : "+v"(b));
+        const int q = nl >> 3, sub = ((nl >> 2) & 1) * 8;
 #pragma unroll
-          for (int i = 0; i < MI; ++i) {
-            const int pl = wm * WM + i * 16 + prow;
-            const f32x4_t a = acc[i][j] + bvv[j];
-            // (scalars, not pk[h] in a loop: hipcc folded the subscripted form into pk[1] = pk[0])
-            uint32_t lo = pack_bf16x2(a[0], a[1]), hi = pack_bf16x2(a[2], a[3]);
-            if (RELU) {
-              lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s16x2_t, lo), (s16x2_t){0, 0}));
-              hi = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s16x2_t, hi), (s16x2_t){0, 0}));
-            }
-            const u32x2_t pk = {lo, hi};
-            *(u32x2_t*)(smem + pl * (BN * 2) + ((q ^ (pl & 7)) << 4) + sub) = pk;
-          }
+        for (int i = 0; i < MI; ++i) {
+          const int pl = wm * WM + i * 16 + prow;
+          const f32x4_t a = acc[i][j] + b;
+          // (scalars, not pk[h] in a loop: hipcc folded the subscripted form into pk[1] = pk[0])
+          uint32_t lo = pack_bf16x2(a[0], a[1]), hi = pack_bf16x2(a[2], a[3]);
+          lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s16x2_t, lo), (s16x2_t){lowest, lowest}));
+          hi = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s16x2_t, hi), (s16x2_t){lowest, lowest}));
+          const u32x2_t pk = {lo, hi};
+          *(u32x2_t*)(smem + pl * (BN * 2) + ((q ^ (pl & 7)) << 4) + sub) = pk;
         }
-      };
-      if (p.relu) body(std::true_type{});
-      else body(std::false_type{});
+      }
     }
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
