@@ -84,8 +84,10 @@ template <class T, int VEC> struct Pack {
   }
 };
 
-// 1 / (1 + exp(-z)).  f32 results: the library's exp and an IEEE division.  16-bit results: the hardware's exp2 and
-// reciprocal (together < 4 units of f32's last place, 2^-13 of a bf16 step).
+// 1 / (1 + exp(-z)).  f32 data: the library's exp and an IEEE division.  16-bit data: the hardware's exp2 and reciprocal,
+// forward 64x56x56x256 bf16 48 us instead of 75, backward 94 instead of 140.  The rounded exponent makes exp(-z) |z| 2^-24 off,
+// exp2 and reciprocal 2^-23 each: the sigmoid is at most 2^-22 off (absolute: |z| s (1 - s) <= 0.23), 2^-12 of f16's step at
+// 1 and 2^-15 of bf16's; dgamma and dbeta are sums, in f32, of terms that are off by so much.
 template <class T> DTP_DEVINL float sigmoid(float z) {
   if constexpr (T::size == 4) return 1.f / (1.f + expf(-z));
   else return __builtin_amdgcn_rcpf(1.f + __expf(-z));

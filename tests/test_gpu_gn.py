@@ -289,7 +289,8 @@ def _check_stats(stats, x, groups, name):
 
 
 STAT_SHAPES = [((2, 56, 56, 64), 16, False), ((3, 14, 14, 60), 12, False), ((2, 30, 31, 8), 1, False), ((2, 5, 7, 33), 3, False),
-               ((2, 128, 128, 64), 1, True), ((1, 301, 257, 24), 4, True), ((1, 200, 200, 9), 3, True)]
+               ((2, 128, 128, 64), 1, True), ((1, 301, 257, 24), 4, True), ((1, 200, 200, 9), 3, True),
+               ((1, 48, 40, 4000), 2, True)]
 
 
 @pytest.mark.parametrize("far", [30.0, 300.0, 1e4, 1e6])
