@@ -1094,7 +1094,9 @@ int ns_chain(const NsCall& c, int steps, const float* coeffs, const float* scale
 
 // One workgroup a matrix: where every m is at most 128 and no long side keeps a single CU busy for longer than the
 // launches it saves.
-// 64 x 576 takes 54 us here and 86 in launches, 64 x 1152 89 and 89; 128 x 128 60 and 89, 128 x 576 128 and 92.
+// 64 x 576 takes 50 us here and 86 in launches, 64 x 1152 89 and 89; 128 x 128 60 and 89, 128 x 576 128 and 92.
+// (All matrices of a part have to be small enough: one that is not takes the others along into the launches, and the
+// last bits of a result depend on the way.)
 bool ns_is_small(const NsCall& c) {
   for (int i = 0; i < c.count; ++i)
     if (c.tb.mat[i].m > 128 || c.tb.mat[i].n > (c.tb.mat[i].m > 64 ? 320 : 1088)) return false;
@@ -1196,9 +1198,12 @@ int fill_table(NsCall& c, int count, const int* rows, const int* cols) {
   return 0;
 }
 
-// A matrix whose products fill the chip by themselves (m above 1024) is worked off alone, the others of a call together:
-// 13.7 ms for all of VGG16's matrices, 18.9 with all 15 in every launch (XCDs whose tiles have a shorter K wait).
-// The parts follow one another on the stream and share the workspace.
+// A matrix with m above 1024 is worked off alone, the others of a call together; the parts follow one another on the stream
+// and share the workspace.  Measured in a list (us; VGG16's thirteen convolution weights and one more, alone / in every
+// launch with them): 1100 x 1100 603 / 664, 1408 x 1408 643 / 806, 2048 x 2048 1179 / 1390,
+// 4096 x 4096 3913 / 5486 (XCDs whose tiles have a shorter K wait for the others).  Where all matrices of a call are alike
+// nothing waits, and the rule costs time: two of 1024 x 1024 414 / 363, three of 1100 x 1100 711 / 528, two of 2048 x 2048
+// 1624 / 1386, of 4096 x 4096 7030 / 7218.
 constexpr int NS_ALONE = 1024;
 
 template <class F> int each_part(const NsCall& all, F run) {

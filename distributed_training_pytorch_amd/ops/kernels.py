@@ -1007,13 +1007,16 @@ def _gn_check(x, groups, act, *vecs):
 
 def _gn_check_writes(dgamma, dbeta, *read):
     """The parameter gradients are written while other workgroups still read: their bytes are nobody else's."""
-    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (dgamma, dbeta) + read]
-    for i in (0, 1):
-        lo, hi = spans[i]
-        for a, b in spans[i + 1:]:
-            if a < hi and lo < b:
-                raise ValueError("gn_bwd: dgamma and dbeta share their memory with each other or with what is read (x, dy, "
-                                 "gamma, beta, stats)")
+    g0, b0 = dgamma.data_ptr(), dbeta.data_ptr()
+    g1, b1 = g0 + dgamma.nbytes, b0 + dbeta.nbytes
+    shared = g0 < b1 and b0 < g1
+    for t in read:
+        lo = t.data_ptr()
+        hi = lo + t.nbytes
+        shared = shared or lo < g1 and g0 < hi or lo < b1 and b0 < hi
+    if shared:
+        raise ValueError("gn_bwd: dgamma and dbeta share their memory with each other or with what is read (x, dy, gamma, "
+                         "beta, stats)")
 
 
 @_functools.lru_cache(maxsize=256)

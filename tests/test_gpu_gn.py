@@ -386,3 +386,17 @@ def test_gn_of_one_channel_and_two_thousand_million_pixels():
     sq = sum((y[0, i:i + part, 0].double() * (x[0, i:i + part, 0].double() - mean) * rstd).sum().item() for i in range(0, hw, part))
     assert abs(dg.item() - sq) <= 4200 * U * sq
     assert dx[0, -100_000:].abs().max().item() <= 8 * 2.0 ** -8 * rstd and dx[0, :100_000].abs().max().item() <= 8 * 2.0 ** -8 * rstd
+
+
+@pytest.mark.parametrize("value", [0.0, 1e4, 3.1415927, -1e-30])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shape,groups,two_passes", STAT_SHAPES)
+def test_gn_of_equal_values(shape, groups, two_passes, dtype, value):
+    """Variance zero: the mean is the value, y is beta, rstd eps^-1/2 (U of its own, U / 2 of eps as an f32)."""
+    k = _k()
+    x = torch.full(shape, value, device="cuda").to(dtype)
+    gamma, beta = torch.full((shape[-1],), 2.0, device="cuda"), torch.linspace(-1, 1, shape[-1], device="cuda")
+    y, stats = k.gn_fwd(x, gamma, beta, groups, act="none")
+    assert (stats[..., 0] == x.view(-1)[0].float()).all()
+    assert (stats[..., 1].double() - 1e-5 ** -0.5).abs().max() <= 1.5 * U * 1e-5 ** -0.5
+    assert torch.equal(y, beta.to(dtype).expand_as(y))
