@@ -147,8 +147,8 @@ struct Deal {
 // Images whose groups fit a workgroup's registers: x is read once and y written once (backward: x and dy read once).
 // A workgroup owns a slab of whole groups of one image: HW rows of TX vectors.  Threads stand in R = NT / TX rows of TX
 // columns, a thread keeps its column and at most KV of its rows.
-// Bound by HBM where it is large (64x56x56x256 bf16 forward 38 us = 5.4 TB/s), by one workgroup's load, fold and store where
-// it is small (4x28x28x512 forward 7.4 us, backward 12.9 of which gn_dparam_kernel 3); backward at 223 registers a lane holds
+// Bound by HBM where it is large (64x56x56x256 bf16 forward 41 us = 5.0 TB/s), by one workgroup's load, fold and store where
+// it is small (4x28x28x512 forward 7.2 us, backward 12.1 of which gn_dparam_kernel 3); backward at 223 registers a lane holds
 // one workgroup a CU, so loads of one do not run under the stores of another (64x28x28x512 43 us, 3.6 TB/s).
 struct GnSlab {
   int SG, slabs;             // groups of a slab, slabs of an image
@@ -459,7 +459,7 @@ __global__ __launch_bounds__(NT) void gn_slab_bwd_kernel(const void* __restrict_
 // Any size: partial sums over pieces of an image, a fold, and a second pass over the data.
 // A block's threads stand in rows of min(C / VEC, 256) columns; a thread keeps its column, so its channels'
 // parameters stay in registers.
-// Bound by HBM and the last-level cache: 64x224x224x64 bf16 forward 73 + 5 + 129 us, 6.0 TB/s; backward 122 + 6 + 209.
+// Bound by HBM and the last-level cache: 64x224x224x64 bf16 forward 75 + 5 + 128 us, 6.0 TB/s; backward 122 + 6 + 209.
 constexpr int GN_T = 256;
 
 // Both passes over data that does not stay in the caches as a whole: the first reads from the front and the second from the
@@ -905,10 +905,10 @@ int slab_fits(const GnShape& s, int vec, int sg, int bwd) {
 // Groups of a slab; 0: none fits, or its rows are so short (64 bytes, 32, 16) that the loads cost more than a second
 // pass.  Rows should be whole cache lines, but every CU should have a workgroup (16x56x56x256 with 256 at least, rows of
 // 32 bytes: forward 16 us, backward 26; with 512, rows of 16: 21 and 41).  Measured (us, slab / two passes; bf16 where
-// nothing else stands, 32 groups): rows of 64 bytes and more always pay (forward 64x56x56x256 38 / 66, backward
-// 64x28x28x512 43 / 58); of 32: forward 32x56x56x256 in f32 36 / 58, backward 32x56x56x256 47 / 55, but backward
-// 64x56x56x256 118 / 90; of 16: forward 8x56x56x256 14 / 19, 16x112x112x128 37 / 43, but 64x112x112x128 179 / 109 and, on
-// half of the CUs, 4x112x112x128 22 / 19; backward 8x56x56x256 23 / 26, but 16x80x80x256 66 / 58.
+// nothing else stands, 32 groups): rows of 64 bytes and more always pay (forward 64x56x56x256 41 / 71, backward
+// 64x28x28x512 43 / 54); of 32: forward 32x56x56x256 in f32 36 / 64, backward 32x56x56x256 46 / 52, but backward
+// 64x56x56x256 119 / 89; of 16: forward 8x56x56x256 14 / 18, 16x112x112x128 38 / 45, but 64x112x112x128 196 / 112 and, on
+// half of the CUs, 4x112x112x128 23 / 19; backward 8x56x56x256 22.5 / 23, but 16x80x80x256 66 / 55.
 int slab_groups(const GnShape& s, int vec, int elem, int bwd, int& threads) {
   const int step = vec / gcd(s.cpg, vec);            // groups that make whole vectors
   const long total = (long)s.N * s.HW * s.C * elem;

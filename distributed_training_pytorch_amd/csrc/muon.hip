@@ -12,8 +12,8 @@
 //
 // Precision.  Q's eigenvalues span a^k (directions that X lacks) to about 1 (those it has): Q X cancels, and a
 // rounding of Q counts a^k times.  Two choices follow.  Segments of at most three steps (5 = 3 + 2): a^3 = 41; one
-// segment of five, a^5 = 484, is 1e-3 off for a matrix of rank one where a loop of f32 products is 5e-5 off, and
-// 3 + 2 is 5e-5 off too.  And every matrix is held as a pair of f16 values, hi + lo (22 bits), scaled by a power of
+// segment of five, a^5 = 484, is 1e-3 off for a matrix of rank one where a loop of f32 products is 8e-5 off, and
+// 3 + 2 is 9e-5 off.  And every matrix is held as a pair of f16 values, hi + lo (22 bits), scaled by a power of
 // two into f16's range; a product of two of them is three MFMA products, hi*hi + hi*lo + lo*hi, accumulated in f32
 // (lo*lo is 2^-22 of the sum).  Single 16-bit values would be 1e-2 and more off.
 //

@@ -118,6 +118,8 @@ __global__ __launch_bounds__(256) void adamw_flat_kernel(float* __restrict__ p, 
 // normalisation affine values, the classifier's head) lie between its matrices, and a captured step must not hold the
 // step number by value.  ranges: per workgroup (first element in the arena, elements, first element in the second
 // moment's own buffer): at most 1024 elements, multiples of 4.  bias corrections 1 - beta^t = -expm1(t ln beta).
+// Bound by memory: 30 bytes an element (28 with a bf16 gradient); VGG16's biases and 1000-class head, 4.1 M elements: 19 us
+// (24 at the rate of a large copy; a loop over one step's data finds part of it in the last-level cache).
 template <bool GRAD_BF16>
 __global__ __launch_bounds__(256) void adamw_ranges_kernel(float* __restrict__ p, const void* __restrict__ g,
                                 float* __restrict__ m, float* __restrict__ v, bf16_t* __restrict__ lp,

@@ -1290,7 +1290,10 @@ def newton_schulz(x, steps=5, coeffs=NS_COEFFS, eps=1e-7, out_dtype=None):
     X = a X + (b S + c S^2) X with S = X X^T (``coeffs`` = a, b, c).  ``x``: [rows, cols], a stack
     [batch, rows, cols], or a list of 2-D tensors of any shapes (one type: f32, bf16 or f16; contiguous);
     returns the same structure in ``out_dtype`` (default: x's).  The products run on pairs of f16 values (22
-    bits), whatever the types: before its rounding the result is as near the exact one as a loop of f32 products'."""
+    bits), whatever the types.  How far an f32 result is from the exact one (2-norm), next to a loop of f32 products:
+    full rank 3e-6 at 64 x 64 (the loop 1.3e-6), 6e-6 at 4150 x 4210 (5e-6); rank one 9e-5 at 64 x 576 (8e-5), 1.2e-4
+    at 1024 x 1024 (2.6e-4), 3e-4 at 4150 x 4210 (5e-4).  Scratch during the call: 12 bytes an element and 20 a
+    min(rows, cols)^2 of up to 24 matrices at once (1.5 GiB for 4096 x 25088), sides rounded up to 64."""
     many = isinstance(x, (list, tuple))
     mats = list(x) if many else [x]
     cf, sc = _ns_check_schedule(steps, coeffs, eps)
@@ -1346,7 +1349,8 @@ def muon_step(params, grads, bufs, lps, lr, momentum=0.95, nesterov=True, weight
 
     s = 0.2 sqrt(max(rows, cols)) ("match_rms_adamw": updates as large as AdamW's, its lr and weight decay carry
     over) or sqrt(max(1, rows / cols)) ("original").  params, bufs: f32; grads: f32 or bf16; lps: bf16 or None for
-    each; all contiguous [rows, cols], no tensor twice."""
+    each; all contiguous [rows, cols], no tensor twice (a gradient may be: it is only read).  Scratch as
+    :func:`newton_schulz`."""
     cf, sc = _ns_check_schedule(steps, coeffs, eps)
     if adjust_lr not in MUON_ADJUST:
         raise ValueError("muon_step: adjust_lr must be one of %s, got %r" % (sorted(MUON_ADJUST), adjust_lr))
