@@ -147,8 +147,8 @@ struct Deal {
 // Images whose groups fit a workgroup's registers: x is read once and y written once (backward: x and dy read once).
 // A workgroup owns a slab of whole groups of one image: HW rows of TX vectors.  Threads stand in R = NT / TX rows of TX
 // columns, a thread keeps its column and at most KV of its rows.
-// Bound by HBM where it is large (64x56x56x256 bf16 forward 41 us = 5.0 TB/s), by one workgroup's load, fold and store where
-// it is small (4x28x28x512 forward 7.2 us, backward 12.1 of which gn_dparam_kernel 3); backward at 223 registers a lane holds
+// Bound by HBM where it is large (64x56x56x256 bf16 forward 42 us = 4.9 TB/s), by one workgroup's load, fold and store where
+// it is small (4x28x28x512 forward 7.5 us, backward 12.1 of which gn_dparam_kernel 3); backward at 223 registers a lane holds
 // one workgroup a CU, so loads of one do not run under the stores of another (64x28x28x512 43 us, 3.6 TB/s).
 struct GnSlab {
   int SG, slabs;             // groups of a slab, slabs of an image
@@ -207,6 +207,13 @@ template <int VEC> DTP_DEVINL void unit_sums(float* a, int u) {
   }
 }
 
+// The unit's first value in each of its places
+template <int VEC> DTP_DEVINL void unit_first(float* a, int u) {
+#pragma unroll
+  for (int e = 1; e < VEC; ++e)
+    if ((e & (u - 1)) != 0) a[e] = a[e - 1];
+}
+
 // f(0), f(1), .. f(N - 1) with the number known where the body is compiled: as a loop, the kept words of some types came to
 // lie in one wide vector, copied at every row's condition (up to 3.5 KB a lane in scratch memory).
 template <class F, int... I> DTP_DEVINL void each_of(F&& f, std::integer_sequence<int, I...>) {
@@ -242,21 +249,29 @@ __global__ __launch_bounds__(NT) void gn_slab_fwd_kernel(const void* __restrict_
   const Deal dealt(s.HW, R);
   const int count = ty < R ? dealt(ty) * u : 0;
   const float inv = count ? 1.f / (float)count : 0.f;
-  float c[VEC], a0[VEC], a1[VEC];
+  // (from the unit's first value: equal values have exactly their own mean, and no sum leaves f32 where the mean does not)
+  float first[VEC], c[VEC], a0[VEC], a1[VEC];
+  if (count) {
+    Pack<T, VEC>::unpack(w[0], first);
+    unit_first<VEC>(first, u);
+  }
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) c[e] = a0[e] = a1[e] = 0.f;
+  for (int e = 0; e < VEC; ++e) {
+    if (!count) first[e] = 0.f;
+    c[e] = a0[e] = a1[e] = 0.f;
+  }
   each<KV>([&](auto i) {
     const int r = ty + i * R;
     if (ty < R && r < s.HW) {
       float f[VEC];
       Pack<T, VEC>::unpack(w[i], f);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) c[e] += f[e];
+      for (int e = 0; e < VEC; ++e) c[e] = fmaf(f[e] - first[e], inv, c[e]);
     }
   });
   unit_sums<VEC>(c, u);
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) c[e] *= inv;        // the thread's mean, or next to it: a0 is what it misses
+  for (int e = 0; e < VEC; ++e) c[e] += first[e];   // the thread's mean, or next to it: a0 is what it misses
   each<KV>([&](auto i) {
     const int r = ty + i * R;
     if (ty < R && r < s.HW) {
@@ -554,7 +569,8 @@ __global__ __launch_bounds__(GN_T) void gn_partial_kernel(const void* __restrict
               for (int e = 0; e < VEC; ++e) {
                 p[e] = 0.f;
 #pragma unroll
-                for (int k = 0; k < GN_RUN; ++k) p[e] = fmaf(f[k][e], 1.f / GN_RUN, p[e]);
+                for (int k = 1; k < GN_RUN; ++k) p[e] = fmaf(f[k][e] - f[0][e], 1.f / GN_RUN, p[e]);
+                p[e] += f[0][e];
               }
             }
             const float all = have + GN_RUN, part = GN_RUN / all, both = have * part;
@@ -905,7 +921,7 @@ int slab_fits(const GnShape& s, int vec, int sg, int bwd) {
 // Groups of a slab; 0: none fits, or its rows are so short (64 bytes, 32, 16) that the loads cost more than a second
 // pass.  Rows should be whole cache lines, but every CU should have a workgroup (16x56x56x256 with 256 at least, rows of
 // 32 bytes: forward 16 us, backward 26; with 512, rows of 16: 21 and 41).  Measured (us, slab / two passes; bf16 where
-// nothing else stands, 32 groups): rows of 64 bytes and more always pay (forward 64x56x56x256 41 / 71, backward
+// nothing else stands, 32 groups): rows of 64 bytes and more always pay (forward 64x56x56x256 42 / 71, backward
 // 64x28x28x512 43 / 54); of 32: forward 32x56x56x256 in f32 36 / 64, backward 32x56x56x256 46 / 52, but backward
 // 64x56x56x256 119 / 89; of 16: forward 8x56x56x256 14 / 18, 16x112x112x128 38 / 45, but 64x112x112x128 196 / 112 and, on
 // half of the CUs, 4x112x112x128 23 / 19; backward 8x56x56x256 22.5 / 23, but 16x80x80x256 66 / 55.

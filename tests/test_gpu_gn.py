@@ -388,7 +388,7 @@ def test_gn_of_one_channel_and_two_thousand_million_pixels():
     assert dx[0, -100_000:].abs().max().item() <= 8 * 2.0 ** -8 * rstd and dx[0, :100_000].abs().max().item() <= 8 * 2.0 ** -8 * rstd
 
 
-@pytest.mark.parametrize("value", [0.0, 1e4, 3.1415927, -1e-30])
+@pytest.mark.parametrize("value", [0.0, 1e4, 3.1415927, -1e-30, 3e38])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("shape,groups,two_passes", STAT_SHAPES)
 def test_gn_of_equal_values(shape, groups, two_passes, dtype, value):
