@@ -5,7 +5,8 @@
 //   backward   dz = dy * act'(z);  dbeta = sum_{n,hw} dz;  dgamma = sum_{n,hw} dz * xhat
 //              dx = rstd * (gamma*dz - m1 - xhat*m2),  m1 = mean_group(gamma*dz),  m2 = mean_group(gamma*dz*xhat)
 //
-// x, y, dy, dx: bf16, f16 or f32; gamma, beta, statistics and a thread's sums: f32; one rounding, of the result.
+// x, y, dy, dx: bf16, f16 or f32; gamma, beta, statistics, a thread's sums, and the backward's sums over threads and over a
+// group's channels: f32; one rounding, of the result.
 // Statistics of an image never leave it, so nothing is shared between images but the gamma / beta gradients, which a last
 // kernel sums in a fixed order (no atomics: results repeat bit for bit).
 //
